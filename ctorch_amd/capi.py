@@ -120,6 +120,11 @@ PROTOTYPES.update({
     "ctamd_log_softmax_backward_cols_f32": [_P, _P, _P, _Z, _Z, _P],
 })
 
+PROTOTYPES.update({
+    "ctamd_group_norm_f32": [_P, _P, _P, C.c_float, C.c_int, _P, _P, _Z, _Z, _Z, _Z, _P],
+    "ctamd_group_norm_backward_f32": [_P, _P, _P, _P, C.c_int, _P, _P, _P, _P, _Z, _Z, _Z, _Z, _P],
+})
+
 _lib = None
 
 

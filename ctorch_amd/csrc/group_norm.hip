@@ -1,0 +1,1049 @@
+// Group normalisation with an activation over [samples, positions, channels] tensors (channels last),
+// and its gradient.  For sample n and group g of w = C / G channels, M = S w values:
+//   mean = 1/M sum x,  var = 1/M sum (x - mean)^2,  rstd = 1 / sqrt(var + eps),
+//   xhat = (x - mean) rstd,  z = xhat weight + bias,  y = act(z)
+//   dz = g act'(z),  dbias = sum_{n,s} dz,  dweight = sum_{n,s} dz xhat,
+//   dx = rstd (dz weight - s1 - xhat s2),  s1 = 1/M sum dz weight,  s2 = 1/M sum dz weight xhat
+// Every step rounds as written (no contraction), so z - and with it ReLU's mask in the gradient - has the
+// bits that the separate operators give from the same statistics.
+//
+// Bound by HBM: 8 bytes per element forward, 12 backward.  Three ways through memory:
+//   rows      one position per sample (a layer's activations): a group is one short run of memory,
+//             owned by 1 - 64 neighbouring lanes; sums are shuffles, everything is read once;
+//   resident  a sample's groups fit the registers of one block: read once, reduced through LDS;
+//   split     a block takes a piece of the positions: a first launch leaves partial sums, a small one
+//             joins them in a fixed order, a last one reads x (and g) again.
+// Variances are formed from deviations from a mean, never as a difference of large sums: each thread
+// takes the mean of the values it holds, then their squared deviations, and parts are joined by
+//   M2 = M2a + M2b + (mean_a - mean_b)^2 na nb / (na + nb),
+// so a group whose mean is large against its deviation keeps its digits.
+#include "common.h"
+#include "devmath.h"
+
+namespace ctamd {
+namespace {
+
+constexpr int kT = 256;
+constexpr int kWaves = kT / 64;
+
+template <int V>
+struct Vec {
+    float v[V];
+};
+template <int V>
+__device__ __forceinline__ Vec<V> load_vec(const float* p) {
+    typedef float vt __attribute__((ext_vector_type(V)));
+    const vt t = *reinterpret_cast<const vt*>(p);
+    Vec<V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = t[i];
+    return r;
+}
+template <>
+__device__ __forceinline__ Vec<1> load_vec<1>(const float* p) { return {{*p}}; }
+template <int V>
+__device__ __forceinline__ void store_vec(float* p, const Vec<V>& a) {
+    typedef float vt __attribute__((ext_vector_type(V)));
+    vt t;
+#pragma unroll
+    for (int i = 0; i < V; ++i) t[i] = a.v[i];
+    *reinterpret_cast<vt*>(p) = t;
+}
+template <>
+__device__ __forceinline__ void store_vec<1>(float* p, const Vec<1>& a) { *p = a.v[0]; }
+template <int V>
+__device__ __forceinline__ Vec<V> affine_vec(const float* p, size_t at, float without) {
+    if (p) return load_vec<V>(p + at);
+    Vec<V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = without;
+    return r;
+}
+
+// 1 / (1 + e^-z) in single precision for any z (e^-z past the largest float gives 0, NaN stays NaN)
+__device__ __forceinline__ float logistic(float z) {
+    const float s = 1.0f + cta_exp_hw(-z);
+    return s > 1e38f ? 0.0f : cta_rcp_refined(s);
+}
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+    if (ACT == CTAMD_ACT_RELU) return z > 0.0f ? z : 0.0f;
+    if (ACT == CTAMD_ACT_SILU) return z * logistic(z);
+    return z;
+}
+// g act'(z); z is only formed where an activation needs it
+template <int ACT>
+__device__ __forceinline__ float activate_grad(float xhat, float w, float b, float g) {
+    if (ACT == CTAMD_ACT_NONE) return g;
+    const float z = xhat * w + b;
+    if (ACT == CTAMD_ACT_RELU) return z > 0.0f ? g : g * 0.0f;
+    const float s = logistic(z);
+    return g * (s * (1.0f + z * (1.0f - s)));
+}
+
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+__device__ __forceinline__ float inv_sqrt(float var, float eps) { return 1.0f / sqrtf(var + eps); }
+
+// ------------------------------------------------------------------------------- rows
+// `lanes` (a power of two, at most 64) neighbouring lanes own one group of one sample, K vectors each.
+template <int V, int K, int ACT>
+__global__ __launch_bounds__(kT) void rows_forward(const float* x, const float* __restrict__ weight, const float* __restrict__ bias,
+                                                   float eps, float* y, float* __restrict__ stats, size_t unit0, size_t units,
+                                                   unsigned groups, unsigned width, unsigned lanes) {
+    const unsigned lane = threadIdx.x & (lanes - 1);
+    const size_t unit = unit0 + size_t(blockIdx.x) * (kT / lanes) + threadIdx.x / lanes;      // sample * groups + group
+    const bool live = unit < units;
+    const unsigned g = unsigned(unit % groups);
+    const float* src = x + unit * width;
+    Vec<V> v[K];
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const unsigned at = (lane + k * lanes) * V;
+        const bool in = live && at < width;
+        v[k] = in ? load_vec<V>(src + at) : Vec<V>{};
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum += v[k].v[i];
+    }
+    const float mean = lanes_sum(sum, int(lanes)) / float(width);
+    float sq = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const bool in = (lane + k * lanes) * V < width;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float d = v[k].v[i] - mean;
+            sq += in ? d * d : 0.0f;
+        }
+    }
+    const float rstd = inv_sqrt(lanes_sum(sq, int(lanes)) / float(width), eps);
+    if (!live) return;
+    if (stats && lane == 0) {
+        stats[2 * unit] = mean;
+        stats[2 * unit + 1] = rstd;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const unsigned at = (lane + k * lanes) * V;
+        if (at < width) {
+            const Vec<V> w = affine_vec<V>(weight, size_t(g) * width + at, 1.0f), b = affine_vec<V>(bias, size_t(g) * width + at, 0.0f);
+            Vec<V> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] = activate<ACT>((v[k].v[i] - mean) * rstd * w.v[i] + b.v[i]);
+            store_vec<V>(y + unit * width + at, o);
+        }
+    }
+}
+
+// The gradient.  A thread keeps its group - and so its channels - over all the samples it visits, and
+// carries their terms of dweight and dbias in registers; the block adds its sample lanes through LDS and
+// leaves one row of partial sums, partials[block][2][C].
+template <int V, int K, int ACT>
+__global__ __launch_bounds__(kT) void rows_backward(const float* x, const float* __restrict__ weight, const float* __restrict__ bias,
+                                                    const float* __restrict__ stats, const float* g_out, float* dx, float* __restrict__ partials,
+                                                    size_t samples, unsigned groups, unsigned width, unsigned lanes, unsigned block_groups,
+                                                    unsigned sample_lanes) {
+    __shared__ float s_red[2 * V][kT];
+    const unsigned lane = threadIdx.x & (lanes - 1), sub = threadIdx.x / lanes;
+    const unsigned g = blockIdx.x * block_groups + sub % block_groups, sl = sub / block_groups;
+    const bool owner = sl < sample_lanes && g < groups;
+    const size_t channels = size_t(groups) * width;
+    Vec<V> w[K], b[K], accw[K], accb[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const unsigned at = (lane + k * lanes) * V;
+        const bool in = owner && at < width;
+        w[k] = in ? affine_vec<V>(weight, size_t(g) * width + at, 1.0f) : Vec<V>{};
+        b[k] = in ? affine_vec<V>(bias, size_t(g) * width + at, 0.0f) : Vec<V>{};
+        accw[k] = Vec<V>{};
+        accb[k] = Vec<V>{};
+    }
+    // every thread of the block makes the same number of turns: the shuffles below want whole waves
+    for (size_t n0 = size_t(blockIdx.y) * sample_lanes; n0 < samples; n0 += size_t(gridDim.y) * sample_lanes) {
+        const size_t n = n0 + sl;
+        const bool live = owner && n < samples;
+        const size_t unit = n * groups + g;
+        const float mean = live ? stats[2 * unit] : 0.0f, rstd = live ? stats[2 * unit + 1] : 0.0f;
+        Vec<V> h[K], d[K];
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const unsigned at = (lane + k * lanes) * V;
+            const bool in = live && at < width;
+            h[k] = in ? load_vec<V>(x + unit * width + at) : Vec<V>{};
+            d[k] = in ? load_vec<V>(g_out + unit * width + at) : Vec<V>{};
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const bool in = live && (lane + k * lanes) * V < width;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float xh = (h[k].v[i] - mean) * rstd;
+                const float dz = in ? activate_grad<ACT>(xh, w[k].v[i], b[k].v[i], d[k].v[i]) : 0.0f;
+                const float t = in ? dz * xh : 0.0f;
+                accb[k].v[i] += dz;
+                accw[k].v[i] += t;
+                h[k].v[i] = xh;
+                d[k].v[i] = dz * w[k].v[i];
+                s1 += d[k].v[i];
+                s2 += t * w[k].v[i];
+            }
+        }
+        if (dx) {
+            s1 = lanes_sum(s1, int(lanes)) / float(width);
+            s2 = lanes_sum(s2, int(lanes)) / float(width);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const unsigned at = (lane + k * lanes) * V;
+                if (live && at < width) {
+                    Vec<V> o;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o.v[i] = (d[k].v[i] - s1 - h[k].v[i] * s2) * rstd;
+                    store_vec<V>(dx + unit * width + at, o);
+                }
+            }
+        }
+    }
+    if (!partials) return;
+    float* row = partials + size_t(blockIdx.y) * 2 * channels;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            s_red[i][threadIdx.x] = accw[k].v[i];
+            s_red[V + i][threadIdx.x] = accb[k].v[i];
+        }
+        __syncthreads();
+        const unsigned at = (lane + k * lanes) * V;
+        if (owner && sl == 0 && at < width) {
+            Vec<V> tw{}, tb{};
+            for (unsigned q = 0; q < sample_lanes; ++q) {
+                const unsigned from = threadIdx.x + q * block_groups * lanes;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    tw.v[i] += s_red[i][from];
+                    tb.v[i] += s_red[V + i][from];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                row[size_t(g) * width + at + i] = tw.v[i];
+                row[channels + size_t(g) * width + at + i] = tb.v[i];
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------- tiles
+// A block covers `cols` vectors of channels (whole groups, or a piece of one group that is wider than
+// the block) and walks the positions `row_lanes` at a time: thread t holds channel vector t % cols of
+// row lane t / cols.  Neighbouring threads read neighbouring memory, and a thread's channels - its
+// weight, its bias, its gradient sums - never change.
+struct Tile {
+    size_t samples, positions, channels;
+    unsigned groups, width;       // channels per group
+    unsigned cols, row_lanes;     // vectors per row of the block, rows at once
+    unsigned block_groups;        // groups per block (1 when pieces > 1)
+    unsigned pieces;              // blocks that share one group
+    unsigned col_blocks;          // blocks along the channels
+    unsigned chunks;              // blocks along the positions (1: resident)
+    size_t chunk_rows;
+};
+struct Place {
+    size_t n;
+    unsigned col_block, chunk, piece;
+    unsigned group0, col0;        // first group, first channel of the block
+    unsigned cols;                // vectors of this block (the last one may have fewer)
+    unsigned col, row;            // this thread's
+    bool live;
+    size_t first, last;           // positions of the chunk
+};
+template <int V, int T>
+__device__ __forceinline__ Place place(const Tile& t, size_t id) {
+    Place p;
+    p.chunk = unsigned(id % t.chunks);
+    id /= t.chunks;
+    p.col_block = unsigned(id % t.col_blocks);
+    p.n = id / t.col_blocks;
+    const unsigned wv = t.width / V;
+    if (t.pieces > 1) {
+        p.piece = p.col_block % t.pieces;
+        p.group0 = p.col_block / t.pieces;
+        p.col0 = p.group0 * t.width + p.piece * t.cols * V;
+        const unsigned rest = wv - p.piece * t.cols;
+        p.cols = rest < t.cols ? rest : t.cols;
+    } else {
+        p.piece = 0;
+        p.group0 = p.col_block * t.block_groups;
+        p.col0 = p.group0 * t.width;
+        const unsigned g = t.groups - p.group0;
+        p.cols = (g < t.block_groups ? g : t.block_groups) * wv;
+    }
+    p.col = threadIdx.x % t.cols;
+    p.row = threadIdx.x / t.cols;
+    p.live = p.row < t.row_lanes && p.col < p.cols;
+    p.first = size_t(p.chunk) * t.chunk_rows;
+    p.last = p.first + t.chunk_rows;
+    if (p.last > t.positions) p.last = t.positions;
+    return p;
+}
+// how many of the rows first, first + step, ... lie before last
+__device__ __forceinline__ size_t rows_of(size_t first, size_t last, unsigned step) {
+    return first < last ? (last - first + step - 1) / step : 0;
+}
+
+struct Moments {
+    float n, mean, m2;
+};
+__device__ __forceinline__ Moments join(const Moments& a, const Moments& b) {
+    Moments r;
+    r.n = a.n + b.n;
+    const float d = b.mean - a.mean, f = r.n > 0.0f ? b.n / r.n : 0.0f;
+    r.mean = a.mean + d * f;
+    r.m2 = a.m2 + b.m2 + d * d * (a.n * f);
+    return r;
+}
+
+// Joins the moments of a block's threads per group; wave w takes the groups w, w + waves, ...  The mean
+// first (a sum of n mean), then the deviations from it.  every(group, moments) is called by lane 0.
+template <int V, int T, class F>
+__device__ __forceinline__ void join_groups(const Tile& t, const Place& p, float* s_mean, float* s_m2, float* s_n, const Moments& mine, F every) {
+    s_mean[threadIdx.x] = mine.mean;
+    s_m2[threadIdx.x] = mine.m2;
+    s_n[threadIdx.x] = p.live ? mine.n : 0.0f;
+    __syncthreads();
+    const unsigned per = t.pieces > 1 ? p.cols : t.width / V;              // vectors of a group in this block
+    const unsigned here = t.pieces > 1 ? 1 : p.cols / per;
+    const unsigned wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const unsigned entries = per * t.row_lanes;
+    for (unsigned g = wave; g < here; g += T / 64) {
+        float n = 0.0f, s = 0.0f;
+        for (unsigned e = lane; e < entries; e += 64) {
+            const unsigned at = (e / per) * t.cols + g * per + e % per;
+            n += s_n[at];
+            s += s_n[at] * s_mean[at];
+        }
+        n = lanes_sum(n, 64);
+        const float mean = n > 0.0f ? lanes_sum(s, 64) / n : 0.0f;
+        float m2 = 0.0f;
+        for (unsigned e = lane; e < entries; e += 64) {
+            const unsigned at = (e / per) * t.cols + g * per + e % per;
+            const float d = s_mean[at] - mean;
+            m2 += s_n[at] > 0.0f ? s_m2[at] + s_n[at] * (d * d) : 0.0f;
+        }
+        m2 = lanes_sum(m2, 64);
+        if (lane == 0) every(g, Moments{n, mean, m2});
+    }
+}
+
+// the moments of the first `count` of K vectors
+template <int V, int K>
+__device__ __forceinline__ Moments moments_of(const Vec<V> (&v)[K], int count) {
+    Moments m{float(count * V), 0.0f, 0.0f};
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) s += k < count ? v[k].v[i] : 0.0f;
+    if (count == 0) return m;
+    m.mean = s / m.n;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float d = v[k].v[i] - m.mean;
+            m.m2 += k < count ? d * d : 0.0f;
+        }
+    return m;
+}
+
+template <int V, int K, int ACT, int T>
+__global__ __launch_bounds__(T) void resident_forward(Tile t, const float* x, const float* __restrict__ weight, const float* __restrict__ bias,
+                                                      float eps, float* y, float* __restrict__ stats) {
+    __shared__ float s_mean[T], s_m2[T], s_n[T];
+    __shared__ float s_stat[T][2];
+    const Place p = place<V, T>(t, blockIdx.x);
+    const float* src = x + (p.n * t.positions + p.row) * t.channels + p.col0 + p.col * V;
+    const size_t step = size_t(t.row_lanes) * t.channels;
+    const int count = p.live ? int(rows_of(p.row, t.positions, t.row_lanes)) : 0;
+    Vec<V> v[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = k < count ? load_vec<V>(src + k * step) : Vec<V>{};
+    const Vec<V> w = p.live ? affine_vec<V>(weight, p.col0 + p.col * V, 1.0f) : Vec<V>{};
+    const Vec<V> b = p.live ? affine_vec<V>(bias, p.col0 + p.col * V, 0.0f) : Vec<V>{};
+    const float whole = float(t.positions * t.width);
+    join_groups<V, T>(t, p, s_mean, s_m2, s_n, moments_of<V, K>(v, count), [&](unsigned g, const Moments& m) {
+        const float rstd = inv_sqrt(m.m2 / whole, eps);
+        s_stat[g][0] = m.mean;
+        s_stat[g][1] = rstd;
+        if (stats) {
+            float* o = stats + 2 * (p.n * t.groups + p.group0 + g);
+            o[0] = m.mean;
+            o[1] = rstd;
+        }
+    });
+    __syncthreads();
+    const unsigned g = p.col / (t.width / V);
+    const float mean = s_stat[g][0], rstd = s_stat[g][1];
+    float* dst = y + (src - x);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (k < count) {
+            Vec<V> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] = activate<ACT>((v[k].v[i] - mean) * rstd * w.v[i] + b.v[i]);
+            store_vec<V>(dst + k * step, o);
+        }
+}
+
+// parts[((n * groups + group) * pieces + piece) * chunks + chunk] = (mean, M2) of that part of the group
+constexpr int kStatRows = 8;
+template <int V>
+__global__ __launch_bounds__(kT) void split_stats(Tile t, const float* __restrict__ x, float* __restrict__ parts) {
+    __shared__ float s_mean[kT], s_m2[kT], s_n[kT];
+    const Place p = place<V, kT>(t, blockIdx.x);
+    Moments run{0.0f, 0.0f, 0.0f};
+    if (p.live) {
+        const float* src = x + (p.n * t.positions + p.first + p.row) * t.channels + p.col0 + p.col * V;
+        const size_t step = size_t(t.row_lanes) * t.channels;
+        size_t left = rows_of(p.first + p.row, p.last, t.row_lanes);
+        for (; left > 0; src += kStatRows * step) {
+            const int count = left < kStatRows ? int(left) : kStatRows;
+            Vec<V> v[kStatRows];
+#pragma unroll
+            for (int k = 0; k < kStatRows; ++k) v[k] = k < count ? load_vec<V>(src + k * step) : Vec<V>{};
+            run = join(run, moments_of<V, kStatRows>(v, count));
+            left -= count;
+        }
+    }
+    join_groups<V, kT>(t, p, s_mean, s_m2, s_n, run, [&](unsigned g, const Moments& m) {
+        float* o = parts + 2 * (((p.n * t.groups + p.group0 + g) * t.pieces + p.piece) * t.chunks + p.chunk);
+        o[0] = m.mean;
+        o[1] = m.m2;
+    });
+}
+
+// One wave per (sample, group): the parts of its chunks and pieces, whose sizes follow from the tile.
+template <int V>
+__global__ __launch_bounds__(kT) void split_join(Tile t, const float* __restrict__ parts, float eps, float* __restrict__ stats) {
+    const size_t unit = size_t(blockIdx.x) * kWaves + (threadIdx.x >> 6);
+    const unsigned lane = threadIdx.x & 63;
+    if (unit >= t.samples * t.groups) return;
+    const unsigned entries = t.pieces * t.chunks;
+    const float* src = parts + 2 * unit * entries;
+    auto size_of = [&](unsigned e) {
+        const unsigned chunk = e % t.chunks, piece = e / t.chunks;
+        const size_t first = size_t(chunk) * t.chunk_rows;
+        size_t rows = t.positions - first;
+        if (rows > t.chunk_rows) rows = t.chunk_rows;
+        unsigned wide = t.width;
+        if (t.pieces > 1) {
+            wide = t.width - piece * t.cols * V;
+            if (wide > t.cols * V) wide = t.cols * V;
+        }
+        return float(rows * wide);
+    };
+    const float whole = float(t.positions * t.width);
+    float s = 0.0f;
+    for (unsigned e = lane; e < entries; e += 64) s += size_of(e) * src[2 * e];
+    const float mean = lanes_sum(s, 64) / whole;
+    float m2 = 0.0f;
+    for (unsigned e = lane; e < entries; e += 64) {
+        const float d = src[2 * e] - mean;
+        m2 += src[2 * e + 1] + size_of(e) * (d * d);
+    }
+    m2 = lanes_sum(m2, 64);
+    if (lane == 0) {
+        stats[2 * unit] = mean;
+        stats[2 * unit + 1] = inv_sqrt(m2 / whole, eps);
+    }
+}
+
+constexpr int kApplyRows = 4;
+template <int V, int ACT>
+__global__ __launch_bounds__(kT) void split_apply(Tile t, const float* x, const float* __restrict__ weight, const float* __restrict__ bias,
+                                                  const float* __restrict__ stats, float* y) {
+    const Place p = place<V, kT>(t, blockIdx.x);
+    if (!p.live) return;
+    const unsigned g = t.pieces > 1 ? 0 : p.col / (t.width / V);
+    const float* st = stats + 2 * (p.n * t.groups + p.group0 + g);
+    const float mean = st[0], rstd = st[1];
+    const Vec<V> w = affine_vec<V>(weight, p.col0 + p.col * V, 1.0f), b = affine_vec<V>(bias, p.col0 + p.col * V, 0.0f);
+    const float* src = x + (p.n * t.positions + p.first + p.row) * t.channels + p.col0 + p.col * V;
+    float* dst = y + (src - x);
+    const size_t step = size_t(t.row_lanes) * t.channels;
+    size_t left = rows_of(p.first + p.row, p.last, t.row_lanes);
+    for (; left > 0; src += kApplyRows * step, dst += kApplyRows * step) {
+        const int count = left < kApplyRows ? int(left) : kApplyRows;
+        Vec<V> v[kApplyRows];
+#pragma unroll
+        for (int k = 0; k < kApplyRows; ++k) v[k] = k < count ? load_vec<V>(src + k * step) : Vec<V>{};
+#pragma unroll
+        for (int k = 0; k < kApplyRows; ++k)
+            if (k < count) {
+                Vec<V> o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o.v[i] = activate<ACT>((v[k].v[i] - mean) * rstd * w.v[i] + b.v[i]);
+                store_vec<V>(dst + k * step, o);
+            }
+        left -= count;
+    }
+}
+
+// Adds the row lanes of a block per channel: the threads of row lane 0 receive the sums of a and b.
+template <int V, int T>
+__device__ __forceinline__ void add_row_lanes(const Tile& t, const Place& p, float (*s_red)[T], Vec<V>& a, Vec<V>& b) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        s_red[i][threadIdx.x] = p.live ? a.v[i] : 0.0f;
+        s_red[V + i][threadIdx.x] = p.live ? b.v[i] : 0.0f;
+    }
+    __syncthreads();
+    if (p.live && p.row == 0) {
+        for (unsigned r = 1; r < t.row_lanes; ++r)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                a.v[i] += s_red[i][threadIdx.x + r * t.cols];
+                b.v[i] += s_red[V + i][threadIdx.x + r * t.cols];
+            }
+    }
+}
+
+// Gradient with a sample's groups in registers.  The block visits the samples blockIdx.y, blockIdx.y +
+// gridDim.y, ... of its channels, carries dweight and dbias, and leaves partials[blockIdx.y][2][C].
+template <int V, int K, int ACT, int T>
+__global__ __launch_bounds__(T) void resident_backward(Tile t, const float* x, const float* __restrict__ weight, const float* __restrict__ bias,
+                                                       const float* __restrict__ stats, const float* g_out, float* dx,
+                                                       float* __restrict__ partials) {
+    __shared__ float s_red[2 * V][T];
+    __shared__ float s_sum[T][2];
+    Place p = place<V, T>(t, blockIdx.x);
+    const unsigned wv = t.width / V, gl = p.col / wv;
+    const Vec<V> w = p.live ? affine_vec<V>(weight, p.col0 + p.col * V, 1.0f) : Vec<V>{};
+    const Vec<V> b = p.live ? affine_vec<V>(bias, p.col0 + p.col * V, 0.0f) : Vec<V>{};
+    const size_t step = size_t(t.row_lanes) * t.channels;
+    const int count = p.live ? int(rows_of(p.row, t.positions, t.row_lanes)) : 0;
+    const float whole = float(t.positions * t.width);
+    const unsigned wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const unsigned here = p.cols / wv, entries = wv * t.row_lanes;
+    Vec<V> accw{}, accb{};
+    for (size_t n = blockIdx.y; n < t.samples; n += gridDim.y) {
+        const size_t at = (n * t.positions + p.row) * t.channels + p.col0 + p.col * V;
+        float mean = 0.0f, rstd = 0.0f;
+        if (p.live) {
+            const float* st = stats + 2 * (n * t.groups + p.group0 + gl);
+            mean = st[0];
+            rstd = st[1];
+        }
+        Vec<V> h[K], d[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            h[k] = k < count ? load_vec<V>(x + at + k * step) : Vec<V>{};
+            d[k] = k < count ? load_vec<V>(g_out + at + k * step) : Vec<V>{};
+        }
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float xh = (h[k].v[i] - mean) * rstd;
+                const float dz = k < count ? activate_grad<ACT>(xh, w.v[i], b.v[i], d[k].v[i]) : 0.0f;
+                const float e = k < count ? dz * xh : 0.0f;
+                accb.v[i] += dz;
+                accw.v[i] += e;
+                h[k].v[i] = xh;
+                d[k].v[i] = dz * w.v[i];
+                s1 += d[k].v[i];
+                s2 += e * w.v[i];
+            }
+        if (dx) {
+            s_red[0][threadIdx.x] = p.live ? s1 : 0.0f;
+            s_red[1][threadIdx.x] = p.live ? s2 : 0.0f;
+            __syncthreads();
+            for (unsigned g = wave; g < here; g += T / 64) {
+                float a1 = 0.0f, a2 = 0.0f;
+                for (unsigned e = lane; e < entries; e += 64) {
+                    const unsigned from = (e / wv) * t.cols + g * wv + e % wv;
+                    a1 += s_red[0][from];
+                    a2 += s_red[1][from];
+                }
+                a1 = lanes_sum(a1, 64);
+                a2 = lanes_sum(a2, 64);
+                if (lane == 0) {
+                    s_sum[g][0] = a1 / whole;
+                    s_sum[g][1] = a2 / whole;
+                }
+            }
+            __syncthreads();
+            s1 = s_sum[gl][0];
+            s2 = s_sum[gl][1];
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (k < count) {
+                    Vec<V> o;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o.v[i] = (d[k].v[i] - s1 - h[k].v[i] * s2) * rstd;
+                    store_vec<V>(dx + at + k * step, o);
+                }
+            __syncthreads();                       // s_red and s_sum are written again for the next sample
+        }
+    }
+    if (!partials) return;
+    add_row_lanes<V, T>(t, p, s_red, accw, accb);
+    if (p.live && p.row == 0) {
+        float* row = partials + size_t(blockIdx.y) * 2 * t.channels + p.col0 + p.col * V;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            row[i] = accw.v[i];
+            row[t.channels + i] = accb.v[i];
+        }
+    }
+}
+
+// parts[(n * chunks + chunk)][2][C]: sums over the chunk's positions of dz xhat and dz, per channel
+constexpr int kGradRows = 4;
+template <int V, int ACT>
+__global__ __launch_bounds__(kT) void split_grad_sums(Tile t, const float* __restrict__ x, const float* __restrict__ weight,
+                                                      const float* __restrict__ bias, const float* __restrict__ stats,
+                                                      const float* __restrict__ g_out, float* __restrict__ parts, size_t n0) {
+    __shared__ float s_red[2 * V][kT];
+    const Place p = place<V, kT>(t, blockIdx.x);
+    Vec<V> sw{}, sb{};
+    if (p.live) {
+        const unsigned gl = t.pieces > 1 ? 0 : p.col / (t.width / V);
+        const float* st = stats + 2 * ((n0 + p.n) * t.groups + p.group0 + gl);
+        const float mean = st[0], rstd = st[1];
+        const Vec<V> w = affine_vec<V>(weight, p.col0 + p.col * V, 1.0f), b = affine_vec<V>(bias, p.col0 + p.col * V, 0.0f);
+        size_t at = ((n0 + p.n) * t.positions + p.first + p.row) * t.channels + p.col0 + p.col * V;
+        const size_t step = size_t(t.row_lanes) * t.channels;
+        size_t left = rows_of(p.first + p.row, p.last, t.row_lanes);
+        for (; left > 0; at += kGradRows * step) {
+            const int count = left < kGradRows ? int(left) : kGradRows;
+            Vec<V> h[kGradRows], d[kGradRows];
+#pragma unroll
+            for (int k = 0; k < kGradRows; ++k) {
+                h[k] = k < count ? load_vec<V>(x + at + k * step) : Vec<V>{};
+                d[k] = k < count ? load_vec<V>(g_out + at + k * step) : Vec<V>{};
+            }
+            Vec<V> tw{}, tb{};                     // a turn's terms first, then the running sum: shorter chains of roundings
+#pragma unroll
+            for (int k = 0; k < kGradRows; ++k)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float xh = (h[k].v[i] - mean) * rstd;
+                    const float dz = activate_grad<ACT>(xh, w.v[i], b.v[i], d[k].v[i]);
+                    tb.v[i] += k < count ? dz : 0.0f;
+                    tw.v[i] += k < count ? dz * xh : 0.0f;
+                }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                sw.v[i] += tw.v[i];
+                sb.v[i] += tb.v[i];
+            }
+            left -= count;
+        }
+    }
+    add_row_lanes<V, kT>(t, p, s_red, sw, sb);
+    if (p.live && p.row == 0) {
+        float* row = parts + (p.n * t.chunks + p.chunk) * 2 * t.channels + p.col0 + p.col * V;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            row[i] = sw.v[i];
+            row[t.channels + i] = sb.v[i];
+        }
+    }
+}
+
+// One wave per (sample, group): the chunks' sums per channel, kept in sums[n][2][C] for dweight and
+// dbias, and the group's s1, s2.
+__global__ __launch_bounds__(kT) void split_grad_join(Tile t, const float* __restrict__ parts, const float* __restrict__ weight,
+                                                      float* __restrict__ sums, float* __restrict__ s12) {
+    const size_t unit = size_t(blockIdx.x) * kWaves + (threadIdx.x >> 6);
+    const unsigned lane = threadIdx.x & 63;
+    if (unit >= t.samples * t.groups) return;
+    const size_t n = unit / t.groups, g = unit % t.groups;
+    float s1 = 0.0f, s2 = 0.0f;
+    for (unsigned c = lane; c < t.width; c += 64) {
+        const size_t ch = g * t.width + c;
+        const float* src = parts + n * t.chunks * 2 * t.channels + ch;
+        float sw = 0.0f, sb = 0.0f;
+        for (unsigned q = 0; q < t.chunks; ++q) {
+            sw += src[size_t(q) * 2 * t.channels];
+            sb += src[(size_t(q) * 2 + 1) * t.channels];
+        }
+        sums[n * 2 * t.channels + ch] = sw;
+        sums[(n * 2 + 1) * t.channels + ch] = sb;
+        const float w = weight ? weight[ch] : 1.0f;
+        s1 += sb * w;
+        s2 += sw * w;
+    }
+    s1 = lanes_sum(s1, 64);
+    s2 = lanes_sum(s2, 64);
+    if (lane == 0) {
+        const float whole = float(t.positions * t.width);
+        s12[2 * unit] = s1 / whole;
+        s12[2 * unit + 1] = s2 / whole;
+    }
+}
+
+template <int V, int ACT>
+__global__ __launch_bounds__(kT) void split_grad_apply(Tile t, const float* x, const float* __restrict__ weight, const float* __restrict__ bias,
+                                                       const float* __restrict__ stats, const float* __restrict__ s12, const float* g_out,
+                                                       float* dx, size_t n0) {
+    const Place p = place<V, kT>(t, blockIdx.x);
+    if (!p.live) return;
+    const unsigned gl = t.pieces > 1 ? 0 : p.col / (t.width / V);
+    const float* st = stats + 2 * ((n0 + p.n) * t.groups + p.group0 + gl);
+    const float mean = st[0], rstd = st[1];
+    const float* ss = s12 + 2 * (p.n * t.groups + p.group0 + gl);
+    const float s1 = ss[0], s2 = ss[1];
+    const Vec<V> w = affine_vec<V>(weight, p.col0 + p.col * V, 1.0f), b = affine_vec<V>(bias, p.col0 + p.col * V, 0.0f);
+    size_t at = ((n0 + p.n) * t.positions + p.first + p.row) * t.channels + p.col0 + p.col * V;
+    const size_t step = size_t(t.row_lanes) * t.channels;
+    size_t left = rows_of(p.first + p.row, p.last, t.row_lanes);
+    for (; left > 0; at += kGradRows * step) {
+        const int count = left < kGradRows ? int(left) : kGradRows;
+        Vec<V> h[kGradRows], d[kGradRows];
+#pragma unroll
+        for (int k = 0; k < kGradRows; ++k) {
+            h[k] = k < count ? load_vec<V>(x + at + k * step) : Vec<V>{};
+            d[k] = k < count ? load_vec<V>(g_out + at + k * step) : Vec<V>{};
+        }
+#pragma unroll
+        for (int k = 0; k < kGradRows; ++k)
+            if (k < count) {
+                Vec<V> o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float xh = (h[k].v[i] - mean) * rstd;
+                    const float dz = activate_grad<ACT>(xh, w.v[i], b.v[i], d[k].v[i]);
+                    o.v[i] = (dz * w.v[i] - s1 - xh * s2) * rstd;
+                }
+                store_vec<V>(dx + at + k * step, o);
+            }
+        left -= count;
+    }
+}
+
+// dweight[c] (+)= sum of partials[r][0][c], dbias likewise from [r][1][c], r in a fixed order: 16 threads
+// take every 16th row of 16 columns, then add through LDS.
+__global__ __launch_bounds__(kT) void grad_columns(const float* __restrict__ partials, size_t rows, size_t channels, float* __restrict__ dweight,
+                                                   float* __restrict__ dbias, int add) {
+    __shared__ float s_part[16][17];
+    const unsigned c = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+    const size_t col = size_t(blockIdx.x) * 16 + c, cols = 2 * channels;
+    float acc[4] = {};
+    if (col < cols) {
+        size_t r = r0;
+        for (; r + 48 < rows; r += 64) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[q] += partials[(r + 16 * q) * cols + col];
+        }
+        for (; r < rows; r += 16) acc[0] += partials[r * cols + col];
+    }
+    s_part[r0][c] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+    __syncthreads();
+    if (threadIdx.x < 16 && col < cols) {
+        float s = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 16; ++q) s += s_part[q][c];
+        float* out = col < channels ? dweight : dbias;
+        if (out) {
+            float* o = out + (col < channels ? col : col - channels);
+            *o = add ? *o + s : s;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------- host side
+unsigned pow2_at_least(unsigned v) {
+    unsigned p = 1;
+    while (p < v) p *= 2;
+    return p;
+}
+
+// how many floats a vector may take: a group starts on it in every row, and every tensor does
+unsigned vector_width(size_t width, std::initializer_list<const void*> ptrs) {
+    uintptr_t bits = 0;
+    for (const void* p : ptrs) bits |= reinterpret_cast<uintptr_t>(p);
+    if (width % 4 == 0 && (bits & 15u) == 0) return 4;
+    if (width % 2 == 0 && (bits & 7u) == 0) return 2;
+    return 1;
+}
+
+constexpr unsigned kRowVectors = 8;             // most vectors a lane holds in the rows kernels
+bool rows_fit(size_t positions, size_t width, unsigned v) { return positions == 1 && width / v <= 64 * kRowVectors; }
+
+// The smallest run of whole groups that fills a 128-byte line in every row, so that a block does not
+// fetch lines it uses a part of - or the whole row, if that is shorter.
+Tile tile_of(size_t n, size_t s, size_t c, unsigned groups, unsigned v, unsigned threads, bool whole_lines_only) {
+    Tile t{};
+    t.samples = n;
+    t.positions = s;
+    t.channels = c;
+    t.groups = groups;
+    t.width = unsigned(c / groups);
+    const unsigned wv = t.width / v;
+    if (wv > threads) {
+        t.pieces = (wv + threads - 1) / threads;
+        t.cols = (wv + t.pieces - 1) / t.pieces;
+        t.pieces = (wv + t.cols - 1) / t.cols;
+        t.block_groups = 1;
+        t.col_blocks = groups * t.pieces;
+    } else {
+        t.pieces = 1;
+        unsigned bg = threads / wv;
+        if (whole_lines_only) {
+            const unsigned want = (32 + t.width - 1) / t.width;
+            if (want < bg) bg = want;
+        }
+        if (bg > groups) bg = groups;
+        t.block_groups = bg;
+        t.cols = bg * wv;
+        t.col_blocks = (groups + bg - 1) / bg;
+    }
+    t.row_lanes = threads / t.cols;
+    t.chunks = 1;
+    t.chunk_rows = s;
+    return t;
+}
+
+// Positions per block of the split kernels: enough blocks for the chip, at least 32 rows of work each
+void split_positions(Tile* t, size_t per_part_floats, size_t floats) {
+    const size_t cus = size_t(compute_units() > 0 ? compute_units() : 256);
+    const size_t want = 8 * cus, others = t->samples * t->col_blocks;
+    size_t chunks = others >= want ? 1 : (want + others - 1) / others;
+    const size_t most = (t->positions + size_t(t->row_lanes) * 16 - 1) / (size_t(t->row_lanes) * 16);
+    if (chunks > most) chunks = most;
+    const size_t room = floats / per_part_floats;       // parts that the scratch holds
+    if (chunks > room) chunks = room;
+    if (chunks < 1) chunks = 1;
+    t->chunk_rows = (t->positions + chunks - 1) / chunks;
+    t->chunks = unsigned((t->positions + t->chunk_rows - 1) / t->chunk_rows);
+}
+
+#define BY_ACT(ACT_VALUE, ...)                                                     \
+    do {                                                                           \
+        if ((ACT_VALUE) == CTAMD_ACT_RELU) { constexpr int ACT = CTAMD_ACT_RELU; __VA_ARGS__; } \
+        else if ((ACT_VALUE) == CTAMD_ACT_SILU) { constexpr int ACT = CTAMD_ACT_SILU; __VA_ARGS__; } \
+        else { constexpr int ACT = CTAMD_ACT_NONE; __VA_ARGS__; }                  \
+    } while (0)
+#define BY_VEC(V_VALUE, ...)                                                       \
+    do {                                                                           \
+        if ((V_VALUE) == 4) { constexpr int V = 4; __VA_ARGS__; }                  \
+        else if ((V_VALUE) == 2) { constexpr int V = 2; __VA_ARGS__; }             \
+        else { constexpr int V = 1; __VA_ARGS__; }                                 \
+    } while (0)
+#define BY_COUNT(K_VALUE, ...)                                                     \
+    do {                                                                           \
+        if ((K_VALUE) <= 1) { constexpr int K = 1; __VA_ARGS__; }                  \
+        else if ((K_VALUE) <= 2) { constexpr int K = 2; __VA_ARGS__; }             \
+        else if ((K_VALUE) <= 4) { constexpr int K = 4; __VA_ARGS__; }             \
+        else { constexpr int K = 8; __VA_ARGS__; }                                 \
+    } while (0)
+
+// Blocks per launch (1024 threads each stay below 2^32); longer batches take several launches.  2^20
+// channels at most, so that one sample's blocks always fit, and its sums fit the scratch.
+constexpr size_t kMostBlocks = size_t(1) << 21;
+constexpr size_t kMostChannels = size_t(1) << 20;
+
+int check_shape(const char* who, size_t batch, size_t positions, size_t channels, size_t groups, int act) {
+    if (groups == 0 || channels % groups != 0) return fail(CTAMD_EINVAL, "%s: %zu channels do not divide into %zu groups", who, channels, groups);
+    if (act != CTAMD_ACT_NONE && act != CTAMD_ACT_RELU && act != CTAMD_ACT_SILU) return fail(CTAMD_EINVAL, "%s: unknown activation %d", who, act);
+    if (channels > kMostChannels) return fail(CTAMD_ERANGE, "%s: more than 2^20 channels", who);
+    if (positions > (size_t(1) << 40) / channels) return fail(CTAMD_ERANGE, "%s: more than 2^40 elements in a sample", who);
+    if (batch > (size_t(1) << 40) / (positions * channels)) return fail(CTAMD_ERANGE, "%s: more than 2^40 elements", who);
+    return CTAMD_OK;
+}
+
+}  // namespace
+}  // namespace ctamd
+
+using namespace ctamd;
+
+extern "C" {
+
+int ctamd_group_norm_f32(const float* x, const float* weight, const float* bias, float eps, int act, float* y, float* stats, size_t batch,
+                         size_t positions, size_t channels, size_t groups, void* stream) {
+    if (batch == 0 || positions == 0 || channels == 0) return CTAMD_OK;
+    int rc = check_shape(__func__, batch, positions, channels, groups, act);
+    if (rc) return rc;
+    if (!x || !y) return fail(CTAMD_EINVAL, "%s: null pointer", __func__);
+    if (!(eps >= 0.0f)) return fail(CTAMD_EINVAL, "%s: eps must not be negative", __func__);
+    hipStream_t s = as_stream(stream);
+    const size_t width = channels / groups;
+    const unsigned v = vector_width(width, {x, y, weight, bias});
+    const double elements = double(batch) * double(positions) * double(channels);
+    if (rows_fit(positions, width, v)) {
+        const unsigned wv = unsigned(width / v), lanes = pow2_at_least(wv < 64 ? wv : 64), count = (wv + lanes - 1) / lanes;
+        const size_t units = batch * groups, per_block = kT / lanes;
+        for (size_t unit0 = 0; unit0 < units; unit0 += kMostBlocks * per_block) {
+            const size_t all = (units - unit0 + per_block - 1) / per_block, blocks = all < kMostBlocks ? all : kMostBlocks;
+            BY_VEC(v, BY_COUNT(count, BY_ACT(act, hipLaunchKernelGGL((rows_forward<V, K, ACT>), dim3(unsigned(blocks)), dim3(kT), 0, s, x, weight, bias,
+                                                                     eps, y, stats, unit0, units, unsigned(groups), unsigned(width), lanes))));
+            rc = launched(__func__);
+            if (rc) return rc;
+        }
+        account(8.0 * elements, 8.0 * elements);
+        return CTAMD_OK;
+    }
+    for (unsigned threads : {256u, 1024u}) {
+        const Tile t = tile_of(batch, positions, channels, unsigned(groups), v, threads, true);
+        const size_t held = (positions + t.row_lanes - 1) / t.row_lanes;
+        if (t.pieces > 1 || held > 8) continue;
+        const size_t slab = kMostBlocks / t.col_blocks;
+        for (size_t n0 = 0; n0 < batch; n0 += slab) {
+            const size_t samples = batch - n0 < slab ? batch - n0 : slab;
+            const unsigned blocks = unsigned(samples * t.col_blocks);
+            const float* xs = x + n0 * positions * channels;
+            float* ys = y + n0 * positions * channels;
+            float* st = stats ? stats + 2 * n0 * groups : nullptr;
+            if (threads == 256)
+                BY_VEC(v, BY_COUNT(held, BY_ACT(act, hipLaunchKernelGGL((resident_forward<V, K, ACT, 256>), dim3(blocks), dim3(256), 0, s, t, xs, weight,
+                                                                        bias, eps, ys, st))));
+            else
+                BY_VEC(v, BY_COUNT(held, BY_ACT(act, hipLaunchKernelGGL((resident_forward<V, K, ACT, 1024>), dim3(blocks), dim3(1024), 0, s, t, xs, weight,
+                                                                        bias, eps, ys, st))));
+            rc = launched(__func__);
+            if (rc) return rc;
+        }
+        account(8.0 * elements, 8.0 * elements);
+        return CTAMD_OK;
+    }
+    ScratchUse use(stream);
+    float* scratch = use.ptr();
+    if (!scratch) return CTAMD_EINVAL;
+    // samples at a time: as many as leave room for a (mean, M2) pair per part and the joined statistics
+    Tile t = tile_of(batch, positions, channels, unsigned(groups), v, kT, false);
+    const size_t per_sample = 2 * groups * (t.pieces + 1);
+    size_t slab = kScratchFloats / per_sample;
+    if (slab > kMostBlocks / t.col_blocks) slab = kMostBlocks / t.col_blocks;
+    if (slab > batch) slab = batch;
+    for (size_t n0 = 0; n0 < batch; n0 += slab) {
+        t.samples = batch - n0 < slab ? batch - n0 : slab;
+        const size_t units = t.samples * groups;
+        split_positions(&t, 2 * units * t.pieces, kScratchFloats - 2 * units);
+        const size_t blocks = t.samples * t.col_blocks * t.chunks;
+        const float* xs = x + n0 * positions * channels;
+        float* ys = y + n0 * positions * channels;
+        float* st = stats ? stats + 2 * n0 * groups : scratch;
+        float* parts = scratch + 2 * units;
+        BY_VEC(v, hipLaunchKernelGGL((split_stats<V>), dim3(unsigned(blocks)), dim3(kT), 0, s, t, xs, parts));
+        rc = launched(__func__);
+        if (rc) return rc;
+        BY_VEC(v, hipLaunchKernelGGL((split_join<V>), dim3(unsigned((units + kWaves - 1) / kWaves)), dim3(kT), 0, s, t, parts, eps, st));
+        rc = launched(__func__);
+        if (rc) return rc;
+        BY_VEC(v, BY_ACT(act, hipLaunchKernelGGL((split_apply<V, ACT>), dim3(unsigned(blocks)), dim3(kT), 0, s, t, xs, weight, bias, st, ys)));
+        rc = launched(__func__);
+        if (rc) return rc;
+    }
+    account(8.0 * elements, 8.0 * elements);
+    return CTAMD_OK;
+}
+
+int ctamd_group_norm_backward_f32(const float* x, const float* weight, const float* bias, const float* stats, int act, const float* g, float* dx,
+                                  float* dweight, float* dbias, size_t batch, size_t positions, size_t channels, size_t groups, void* stream) {
+    if (channels == 0 || (!dx && !dweight && !dbias)) return CTAMD_OK;
+    if (batch == 0 || positions == 0) {
+        int rc = dweight ? ctamd_fill_f32(dweight, 0.0f, channels, stream) : CTAMD_OK;
+        return rc || !dbias ? rc : ctamd_fill_f32(dbias, 0.0f, channels, stream);
+    }
+    int rc = check_shape(__func__, batch, positions, channels, groups, act);
+    if (rc) return rc;
+    if (!x || !stats || !g) return fail(CTAMD_EINVAL, "%s: null pointer", __func__);
+    hipStream_t s = as_stream(stream);
+    const size_t width = channels / groups;
+    const unsigned v = vector_width(width, {x, g, dx, weight, bias});
+    const size_t cus = size_t(compute_units() > 0 ? compute_units() : 256);
+    const double elements = double(batch) * double(positions) * double(channels);
+    const bool columns = dweight || dbias;
+    ScratchUse use(stream);
+    float* scratch = use.ptr();
+    if (!scratch) return CTAMD_EINVAL;
+    const size_t most_rows = kScratchFloats / (2 * channels);           // rows of partial sums that the scratch holds (at least 2)
+    auto fold = [&](const float* partials, size_t rows, int add) {
+        hipLaunchKernelGGL(grad_columns, dim3(unsigned((2 * channels + 15) / 16)), dim3(kT), 0, s, partials, rows, channels, dweight, dbias, add);
+        return launched("ctamd_group_norm_backward_f32");
+    };
+    if (rows_fit(positions, width, v)) {
+        const unsigned wv = unsigned(width / v), lanes = pow2_at_least(wv < 64 ? wv : 64), count = (wv + lanes - 1) / lanes;
+        const unsigned subs = kT / lanes, block_groups = groups < subs ? unsigned(groups) : subs, sample_lanes = subs / block_groups;
+        const size_t col_blocks = (groups + block_groups - 1) / block_groups;
+        size_t blocks = (batch + sample_lanes - 1) / sample_lanes, want = 4 * cus / col_blocks;
+        if (want < 1) want = 1;
+        if (blocks > want) blocks = want;
+        if (blocks > most_rows) blocks = most_rows;
+        if (blocks > 65535) blocks = 65535;
+        BY_VEC(v, BY_COUNT(count, BY_ACT(act, hipLaunchKernelGGL((rows_backward<V, K, ACT>), dim3(unsigned(col_blocks), unsigned(blocks)), dim3(kT), 0,
+                                                                 s, x, weight, bias, stats, g, dx, columns ? scratch : nullptr, batch,
+                                                                 unsigned(groups), unsigned(width), lanes, block_groups, sample_lanes))));
+        rc = launched(__func__);
+        if (!rc && columns) rc = fold(scratch, blocks, 0);
+        if (!rc) account(12.0 * elements, 16.0 * elements);
+        return rc;
+    }
+    for (unsigned threads : {256u, 1024u}) {
+        const Tile t = tile_of(batch, positions, channels, unsigned(groups), v, threads, true);
+        const size_t held = (positions + t.row_lanes - 1) / t.row_lanes;
+        if (t.pieces > 1 || held > (threads == 256 ? 8 : 4)) continue;
+        size_t rows = 4 * cus * 256 / threads / t.col_blocks;
+        if (rows < 1) rows = 1;
+        if (rows > batch) rows = batch;
+        if (rows > most_rows) rows = most_rows;
+        if (rows > 65535) rows = 65535;
+        const dim3 grid(t.col_blocks, unsigned(rows));
+        float* partials = columns ? scratch : nullptr;
+        if (threads == 256)
+            BY_VEC(v, BY_COUNT(held, BY_ACT(act, hipLaunchKernelGGL((resident_backward<V, K, ACT, 256>), grid, dim3(256), 0, s, t, x, weight, bias, stats,
+                                                                    g, dx, partials))));
+        else if (held > 2)
+            BY_VEC(v, BY_ACT(act, hipLaunchKernelGGL((resident_backward<V, 4, ACT, 1024>), grid, dim3(1024), 0, s, t, x, weight, bias, stats, g, dx,
+                                                     partials)));
+        else
+            BY_VEC(v, BY_ACT(act, hipLaunchKernelGGL((resident_backward<V, 2, ACT, 1024>), grid, dim3(1024), 0, s, t, x, weight, bias, stats, g, dx,
+                                                     partials)));
+        rc = launched(__func__);
+        if (!rc && columns) rc = fold(scratch, rows, 0);
+        if (!rc) account(12.0 * elements, 16.0 * elements);
+        return rc;
+    }
+    Tile t = tile_of(batch, positions, channels, unsigned(groups), v, kT, false);
+    // per sample: its channels' sums, s1 and s2 per group, and one part at least
+    const size_t per_sample = 2 * channels + 2 * groups;
+    size_t slab = kScratchFloats / (per_sample + 2 * channels);
+    if (slab > kMostBlocks / t.col_blocks) slab = kMostBlocks / t.col_blocks;
+    if (slab > batch) slab = batch;
+    for (size_t n0 = 0; n0 < batch; n0 += slab) {
+        t.samples = batch - n0 < slab ? batch - n0 : slab;
+        split_positions(&t, 2 * channels * t.samples, kScratchFloats - t.samples * per_sample);
+        const size_t blocks = t.samples * t.col_blocks * t.chunks, units = t.samples * groups;
+        float* sums = scratch;
+        float* s12 = sums + t.samples * 2 * channels;
+        float* parts = s12 + 2 * units;
+        BY_VEC(v, BY_ACT(act, hipLaunchKernelGGL((split_grad_sums<V, ACT>), dim3(unsigned(blocks)), dim3(kT), 0, s, t, x, weight, bias, stats, g, parts, n0)));
+        rc = launched(__func__);
+        if (rc) return rc;
+        hipLaunchKernelGGL(split_grad_join, dim3(unsigned((units + kWaves - 1) / kWaves)), dim3(kT), 0, s, t, parts, weight, sums, s12);
+        rc = launched(__func__);
+        if (rc) return rc;
+        if (dx) {
+            BY_VEC(v, BY_ACT(act, hipLaunchKernelGGL((split_grad_apply<V, ACT>), dim3(unsigned(blocks)), dim3(kT), 0, s, t, x, weight, bias, stats, s12, g,
+                                                     dx, n0)));
+            rc = launched(__func__);
+            if (rc) return rc;
+        }
+        if (columns) {
+            rc = fold(sums, t.samples, n0 > 0);
+            if (rc) return rc;
+        }
+    }
+    account(12.0 * elements, 16.0 * elements);
+    return CTAMD_OK;
+}
+
+}  // extern "C"

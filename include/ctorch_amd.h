@@ -294,6 +294,34 @@ int ctamd_linear_ce_head_f32(const float* h, const float* w, const float* bias, 
                              float* z, float* dz, float* dh, int mask_by_h, float* gw, float* gb, size_t batch, size_t hidden,
                              size_t classes, void* stream);
 
+/* ------------------------------------------------------------------------ normalised layers */
+/* Group normalisation with an activation.  x and y are [batch, positions, channels], channels last; the
+ * channels divide into `groups` runs of channels / groups neighbours, and every (sample, group) is
+ * normalised over its positions * channels / groups values:
+ *   xhat = (x - mean) * rstd,  rstd = 1 / sqrt(var + eps),  var = the mean of (x - mean)^2,
+ *   y = act(xhat * weight[c] + bias[c])
+ * weight and bias are [channels]; NULL stands for ones and zeros.  groups == 1 and positions == 1 is layer
+ * normalisation, groups == channels instance normalisation.  act: CTAMD_ACT_NONE, CTAMD_ACT_RELU
+ * (z > 0 ? z : +0, as ctamd_relu_f32), CTAMD_ACT_SILU (z / (1 + e^-z), within 4 ulp).  stats (may be
+ * NULL) receives (mean, rstd) per sample and group, [batch, groups, 2]: what the gradient reads.  y may be
+ * x.  The variance is formed from deviations from a mean (never as a difference of large sums), sums are
+ * fp32 trees in a fixed order: the same call gives the same bits.  Up to 2^20 channels and 2^40 elements
+ * (CTAMD_ERANGE beyond); groups that do not divide the channels are CTAMD_EINVAL.  Uses the per-device
+ * scratch.  No counterpart in the reference, whose layers are linear + ReLU (mnist/mnist.cpp:39-41);
+ * stands between its Add and ReLU kernels. */
+enum { CTAMD_ACT_NONE = 0, CTAMD_ACT_RELU = 1, CTAMD_ACT_SILU = 2 };
+int ctamd_group_norm_f32(const float* x, const float* weight, const float* bias, float eps, int act, float* y, float* stats,
+                         size_t batch, size_t positions, size_t channels, size_t groups, void* stream);
+/* Its gradient from the upstream gradient g of y's shape and the statistics that the forward pass left:
+ *   dz = g * act'(z),  dbias = sum dz,  dweight = sum dz * xhat  (over samples and positions),
+ *   dx = (dz * weight - s1 - xhat * s2) * rstd,  s1, s2 the group's means of dz * weight and dz * weight * xhat
+ * z is formed again with the forward pass's roundings, so ReLU's mask is the forward pass's.  dx, dweight,
+ * dbias may each be NULL (not wanted); dx may be g or x.  batch == 0 or positions == 0 leaves
+ * dweight and dbias zero.  Uses the per-device scratch; deterministic. */
+int ctamd_group_norm_backward_f32(const float* x, const float* weight, const float* bias, const float* stats, int act,
+                                  const float* g, float* dx, float* dweight, float* dbias, size_t batch, size_t positions,
+                                  size_t channels, size_t groups, void* stream);
+
 /* -------------------------------------------------------------------------------- matmul */
 /* C[i,j] = sum_l A[i*as0 + l*as1] * B[l*bs0 + j*bs1]; C is [m, n] row-major contiguous; strides
  * are in elements and may describe a transposed view.  MatMul_BASIC_kernel.cpp:42-54.  The
