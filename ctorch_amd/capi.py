@@ -125,6 +125,26 @@ PROTOTYPES.update({
     "ctamd_group_norm_backward_f32": [_P, _P, _P, _P, C.c_int, _P, _P, _P, _P, _Z, _Z, _Z, _Z, _P],
 })
 
+PROTOTYPES.update({
+    "ctamd_newton_schulz_workspace": [_I64, _I64, _I64, C.POINTER(_Z)],
+    "ctamd_newton_schulz_f32": [_P, _P, _I64, _I64, _I64, C.c_int, C.POINTER(C.c_float), C.c_float, _P, _Z, _P],
+    "ctamd_muon_workspace": [_P, C.c_int, C.POINTER(_Z)],
+    "ctamd_muon_step_f32": [_P, C.c_int, _P, _P, _Z, _P],
+})
+
+
+class MuonMatrix(C.Structure):
+    """ctamd_muon_matrix"""
+    _fields_ = [("param", _P), ("grad", _P), ("momentum", _P), ("new_param", _P), ("new_momentum", _P), ("rows", _I64), ("cols", _I64),
+                ("scale", C.c_float)]
+
+
+class MuonOptions(C.Structure):
+    """ctamd_muon_options"""
+    _fields_ = [("learning_rate", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float), ("eps", C.c_float),
+                ("nesterov", C.c_int32), ("steps", C.c_int32), ("coefficients", C.c_float * 3)]
+
+
 _lib = None
 
 

@@ -366,6 +366,53 @@ int ctamd_matmul_colsum_f32(const float* a, int64_t as0, int64_t as1, const floa
 int ctamd_matmul_relu_mask_f32(const float* a, int64_t as0, int64_t as1, const float* b, int64_t bs0, int64_t bs1,
                                const float* y, float* c, int64_t m, int64_t n, int64_t k, void* stream);
 
+/* --------------------------------------------------------------------- orthogonalised updates */
+/* out = the matrix g [rows, cols] with its singular values driven towards one, by Newton-Schulz products:
+ *   X = g / (|g|_F + eps), then `steps` times  A = X X^T,  X = a X + (b A + c A A) X
+ * (for rows > cols on the transposed matrix; the result is the same), `batch` matrices one after the other
+ * in memory.  coefficients_host (HOST, may be NULL): a, b, c; NULL stands for 3.4445, -4.7750, 2.0315, which
+ * in 5 steps take singular values of 0.005 |g|_F and more to 0.7 - 1.2.  Matrices are held as pairs of f16
+ * numbers with 22 bits together and multiplied by the f16 matrix cores with fp32 sums: as close to the
+ * iteration in 64 bits as fp32 products are.  That holds while the entries of X stay below 8 and
+ * those of A and b A + c A A below 32 (singular values below 4 or so; the given coefficients keep them below
+ * 1.3); coefficients beyond 32 are CTAMD_EINVAL.  An update whose norm is far below eps comes out as zero
+ * to within 2^-30.  out may be g.  rows and cols up to 2^20, the shorter up to 2^15 (CTAMD_ERANGE).
+ * workspace: at least the bytes that ctamd_newton_schulz_workspace stores in bytes_host (HOST), 16-byte
+ * aligned, not shared by calls that overlap - graphs that may replay at the same time included; nothing in
+ * it is kept from one call to the next.  Deterministic: the same call gives the same bits.  No counterpart
+ * in the reference, whose optimiser is plain gradient descent (mnist/mnist.cpp:86-93). */
+int ctamd_newton_schulz_workspace(int64_t rows, int64_t cols, int64_t batch, size_t* bytes_host);
+int ctamd_newton_schulz_f32(const float* g, float* out, int64_t rows, int64_t cols, int64_t batch, int steps,
+                            const float* coefficients_host, float eps, void* workspace, size_t workspace_bytes, void* stream);
+/* One optimiser step with orthogonalised momentum for `count` weight matrices (HOST table of device
+ * pointers, read before the call returns):
+ *   new_momentum = momentum' = options.momentum * momentum + grad
+ *   U = options.nesterov ? grad + options.momentum * momentum' : momentum'
+ *   new_param = param * (1 - learning_rate * weight_decay) - learning_rate * scale * orthogonalised(U)
+ * with the iteration of ctamd_newton_schulz_f32 (options.steps, coefficients, eps).  new_param may be param
+ * and new_momentum may be momentum (an update in place); no other two tensors may overlap.  scale is the
+ * matrix's own factor, e.g. 0.2 * sqrt(max(rows, cols)) for updates as large as an adaptive optimiser's.
+ * The matrices of a call share its launches (16 at a time).  Workspace as above, from
+ * ctamd_muon_workspace.  Stands beside ctamd_sgd_step_multi_f32 for weight matrices; biases and other
+ * vectors stay with that. */
+typedef struct ctamd_muon_matrix {
+    const float* param;
+    const float* grad;
+    const float* momentum;
+    float* new_param;
+    float* new_momentum;
+    int64_t rows, cols;
+    float scale;
+} ctamd_muon_matrix;
+typedef struct ctamd_muon_options {
+    float learning_rate, momentum, weight_decay, eps;
+    int32_t nesterov, steps;
+    float coefficients[3];
+} ctamd_muon_options;
+int ctamd_muon_workspace(const ctamd_muon_matrix* matrices, int count, size_t* bytes_host);
+int ctamd_muon_step_f32(const ctamd_muon_matrix* matrices, int count, const ctamd_muon_options* options, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 /* -------------------------------------------------------------------------- comparisons */
 /* out[i] = (a[i] cmp b[i]) or (a[i] cmp s) as one byte, 0 or 1 - the reference's bool tensors.
  * Tensor::operator>,<,==,>=,<=,!=(float) src/Tensor.cpp:985-1116 and (const Tensor&) :1119-1309;
