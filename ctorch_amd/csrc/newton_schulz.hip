@@ -13,11 +13,12 @@
 // the polynomial's slope at zero, a^steps, magnifies any rounding of the first steps alike.
 //
 // Layout of a matrix of pairs: row-major, rows padded to 64 columns (zeros), each run of 8 columns stored as
-// [8 hi][8 lo], 32 bytes.  A k step of 32 is 128 bytes of a row, one cache line, and goes to LDS by the
-// direct-to-LDS load; 16-byte units are permuted by the row's low bits so that the fragment reads (one
-// ds_read_b128 per 32 x 16 operand half) meet no bank twice.  Both operands of every product are read
+// [8 hi][8 lo], 32 bytes.  A k step of 16 is 64 bytes of a row and goes to LDS by the direct-to-LDS load;
+// 16-byte units are permuted by bits 2 and 3 of the row, so that the 16 lanes that the 64 banks serve at
+// once (of a ds_read_b128 per 32 x 16 operand half) meet no bank twice.  Both operands of every product are read
 // along their rows (A and B are symmetric; X is kept with its transpose Y), so one kernel serves all three.
 #include <cmath>
+#include <type_traits>
 
 #include "common.h"
 
@@ -36,7 +37,7 @@ constexpr int kXcds = 8;
 constexpr float kScaleX = 8192.0f, kScaleA = 2048.0f;
 
 constexpr int kMaxJobs = 16;
-constexpr int kNormParts = 256;
+constexpr int kNormParts = 1024;
 
 // One matrix - or `count` matrices of one shape, `stride` elements apart - of a call.
 struct Job {
@@ -52,6 +53,7 @@ struct Job {
     unsigned count;
     int tall;                    // rows > cols: X is the transposed update
     float step;                  // learning rate times the matrix's scale
+    int vec;                     // every tensor and every row allows vectors of 4
     unsigned norm_parts;
     size_t part_size;            // elements per part of the norm
 };
@@ -96,21 +98,36 @@ __global__ __launch_bounds__(kThreads) void momentum_norm(Table t) {
     size_t last = first + j.part_size;
     if (last > elements) last = elements;
     const float* g = j.grad + item * j.stride;
+    const float* mo = j.momentum ? j.momentum + item * j.stride : nullptr;
+    float* mn = j.momentum ? j.new_momentum + item * j.stride : nullptr;
     double sum = 0.0;
-    if (j.momentum) {
-        const float* mo = j.momentum + item * j.stride;
-        float* mn = j.new_momentum + item * j.stride;
-        for (size_t i = first + threadIdx.x; i < last; i += kThreads) {
-            const float gi = g[i], m = t.mu * mo[i] + gi;
+    size_t i = first + threadIdx.x;
+    if (j.vec) {                                     // part sizes are multiples of 4
+        for (size_t v = first + size_t(threadIdx.x) * 4; v + 4 <= last; v += kThreads * 4) {
+            v4f u = *reinterpret_cast<const v4f*>(g + v);
+            if (mo) {
+                const v4f old = *reinterpret_cast<const v4f*>(mo + v);
+                v4f m;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    m[e] = t.mu * old[e] + u[e];
+                    u[e] = t.nesterov ? u[e] + t.mu * m[e] : m[e];
+                }
+                *reinterpret_cast<v4f*>(mn + v) = m;
+            }
+            const double d0 = u[0], d1 = u[1], d2 = u[2], d3 = u[3];
+            sum += (d0 * d0 + d1 * d1) + (d2 * d2 + d3 * d3);
+        }
+        i = last - (last - first) % 4 + threadIdx.x;
+    }
+    for (; i < last; i += kThreads) {
+        float u = g[i];
+        if (mo) {
+            const float m = t.mu * mo[i] + u;
             mn[i] = m;
-            const double u = t.nesterov ? gi + t.mu * m : m;
-            sum += u * u;
+            u = t.nesterov ? u + t.mu * m : m;
         }
-    } else {
-        for (size_t i = first + threadIdx.x; i < last; i += kThreads) {
-            const double u = g[i];
-            sum += u * u;
-        }
+        sum += double(u) * double(u);
     }
     sum = block_sum(sum, s_part);
     if (threadIdx.x == 0) reinterpret_cast<double*>(j.work + item * j.work_stride)[part] = sum;
@@ -119,11 +136,10 @@ __global__ __launch_bounds__(kThreads) void momentum_norm(Table t) {
 // 1 / (|U|_F + eps) from the parts; every thread gets it.  Kept in double: its product with an element of U
 // is rounded once, and a norm of 1e38 has an inverse.
 __device__ __forceinline__ double inverse_norm(const Table& t, const Job& j, const char* work, double* s_part) {
-    const double v = threadIdx.x < j.norm_parts ? reinterpret_cast<const double*>(work)[threadIdx.x] : 0.0;
+    double v = 0.0;
+    for (unsigned i = threadIdx.x; i < j.norm_parts; i += kThreads) v += reinterpret_cast<const double*>(work)[i];
     return 1.0 / (sqrt(block_sum(v, s_part)) + double(t.eps));
 }
-static_assert(kNormParts <= kThreads, "a thread per part");
-
 __device__ __forceinline__ float update_at(const Table& t, const Job& j, size_t i) {
     if (!j.momentum) return j.grad[i];
     const float m = j.new_momentum[i];
@@ -158,12 +174,28 @@ __global__ __launch_bounds__(kThreads) void load_pairs(Table t) {
     for (int q = 0; q < 2; ++q) {
         const unsigned r = (threadIdx.x >> 3) + 32 * q, c = (threadIdx.x & 7) * 8;
         float v[8];
+        const size_t at = item * j.stride + size_t(r0 + r) * j.cols + c0 + c;
+        if (j.vec && int64_t(r0 + r) < j.rows && int64_t(c0 + c + 8) <= j.cols) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const bool in = int64_t(r0 + r) < j.rows && int64_t(c0 + c + e) < j.cols;
-            v[e] = in ? float(update_at(t, j, item * j.stride + size_t(r0 + r) * j.cols + c0 + c + e) * inv) : 0.0f;
-            s_tile[r][c + e] = v[e];
+            for (int h = 0; h < 2; ++h) {
+                v4f u = *reinterpret_cast<const v4f*>((j.momentum && !t.nesterov ? j.new_momentum : j.grad) + at + 4 * h);
+                if (j.momentum && t.nesterov) {
+                    const v4f m = *reinterpret_cast<const v4f*>(j.new_momentum + at + 4 * h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) u[e] = u[e] + t.mu * m[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * h + e] = float(u[e] * inv);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const bool in = int64_t(r0 + r) < j.rows && int64_t(c0 + c + e) < j.cols;
+                v[e] = in ? float(update_at(t, j, at + e) * inv) : 0.0f;
+            }
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s_tile[r][c + e] = v[e];
         h8 hi, lo;
         split8(v, kScaleX, &hi, &lo);
         h8* dst = reinterpret_cast<h8*>(straight + (size_t(r0 + r) * cp + c0 + c) * 4);
@@ -210,15 +242,22 @@ __global__ __launch_bounds__(kThreads) void scaled_update(Table t) {
 // written as the call's result.
 enum Kind { GRAM, POLY, STEP, LAST };
 
-template <int BT_, int WM_, int WN_>
+// A block computes a BT x BT tile.  Its waves stand in (BT / WM) x (BT / WN) positions, KG waves to a
+// position, and those share the k range: a stage of the ring is F slabs of 16 k, wave group g multiplies
+// the slabs g, g + KG, ...  (a large wave tile reads each fragment from LDS for more MFMAs; on a small
+// block tile only the k range is left to share).  RING stages, all but one on their way.
+template <int BT_, int WM_, int WN_, int KG_, int F_, int RING_>
 struct TileCfg {
-    static constexpr int BT = BT_, WM = WM_, WN = WN_;         // square block tile, wave tile
+    static constexpr int BT = BT_, WM = WM_, WN = WN_, KG = KG_, F = F_, RING = RING_;
     static constexpr int TM = WM / 32, TN = WN / 32;
-    static constexpr int WAVES = (BT / WM) * (BT / WN), THREADS = WAVES * 64;
-    static constexpr int BUF = 2 * BT * 128;                   // bytes of one k step of both operands
-    static constexpr int LOADS = 2 * BT / (WAVES * 8);         // direct-to-LDS loads per wave and k step
-    static_assert(BT % (WAVES * 8) == 0, "a load does not straddle the operands");
-    static_assert(WAVES * 4096 <= BUF, "the epilogue turns a 32 x 32 tile per wave in one buffer");
+    static constexpr int POSITIONS = (BT / WM) * (BT / WN), WAVES = POSITIONS * KG, THREADS = WAVES * 64;
+    static constexpr int UNITS = 2 * BT / 16;                  // loads of a wave (16 rows x 64 bytes) in a slab
+    static constexpr int SLAB = 2 * BT * 64, STAGE = F * SLAB; // bytes
+    static constexpr int LOADS = F * UNITS / WAVES;            // loads per wave and stage
+    static_assert(F * UNITS % WAVES == 0 && (UNITS % WAVES == 0 || WAVES % UNITS == 0), "the waves share a stage's loads evenly");
+    static_assert(F % KG == 0 && (RING == 3 || RING == 4), "");
+    static_assert(WAVES * 4096 <= RING * STAGE, "the epilogue turns a 32 x 32 tile per wave in the ring");
+    static_assert((KG - 1) * BT * BT * 4 <= RING * STAGE, "the groups' sums meet in the ring");
 };
 
 __device__ __forceinline__ void lds_load(const char* g, char* l) {
@@ -227,8 +266,11 @@ __device__ __forceinline__ void lds_load(const char* g, char* l) {
 
 template <class C, Kind KIND>
 __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, float ca, float cb, float cc) {
-    __shared__ __attribute__((aligned(128))) char s_buf0[C::BUF];
-    __shared__ __attribute__((aligned(128))) char s_buf1[C::BUF];
+    // arrays of their own, so that the compiler can tell a load into one from reads of another
+    __shared__ __attribute__((aligned(128))) char s_ring0[C::STAGE];
+    __shared__ __attribute__((aligned(128))) char s_ring1[C::STAGE];
+    __shared__ __attribute__((aligned(128))) char s_ring2[C::STAGE];
+    __shared__ __attribute__((aligned(128))) char s_ring3[C::RING == 4 ? C::STAGE : 16];
     const int which = job_of(t, blockIdx.x);
     const Job& j = t.job[which];
     const unsigned here = t.first[which + 1] - t.first[which];
@@ -260,26 +302,30 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
     const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     // this lane's byte offset of every load, from the operand's first row of the tile; rows beyond the matrix
     // read its last one (their results are not stored)
+    constexpr unsigned kHalf = C::BT / 16;           // units of the first operand in a slab
     unsigned off[C::LOADS];
 #pragma unroll
     for (int l = 0; l < C::LOADS; ++l) {
-        unsigned r = unsigned(l) * C::WAVES * 8 + wave * 8 + (lane >> 3);
-        const bool second = l >= C::LOADS / 2;
-        if (second) r -= C::BT;
+        const unsigned u = unsigned(l) * C::WAVES + wave, slab = u / C::UNITS, unit = u % C::UNITS;
+        const bool second = unit >= kHalf;
+        unsigned r = (second ? unit - kHalf : unit) * 16 + (lane >> 2);
         const unsigned most = (second ? rows_q - j0 : rows_p - i0) - 1;
         if (r > most) r = most;
-        off[l] = r * k * 4 + ((lane & 7) ^ (lane >> 3)) * 16;
+        off[l] = r * k * 4 + slab * 64 + ((lane & 3) ^ (lane >> 4 & 3)) * 16;
     }
     const char* pb = p + size_t(i0) * k * 4;
     const char* qb = q + size_t(j0) * k * 4;
-    auto load = [&](char* buf, unsigned step) {
+    auto load = [&](char* buf, unsigned stage) {
 #pragma unroll
-        for (int l = 0; l < C::LOADS; ++l)
-            lds_load((l < C::LOADS / 2 ? pb : qb) + size_t(step) * 128 + off[l], buf + (l * C::WAVES + wave) * 1024);
+        for (int l = 0; l < C::LOADS; ++l) {
+            const unsigned u = unsigned(l) * C::WAVES + wave;
+            lds_load((u % C::UNITS < kHalf ? pb : qb) + size_t(stage) * (C::F * 64) + off[l], buf + u * 1024);
+        }
         __builtin_amdgcn_sched_barrier(0);
     };
 
-    const unsigned wm = (wave / (C::BT / C::WN)) * C::WM, wn = (wave % (C::BT / C::WN)) * C::WN;
+    const unsigned group = wave / C::POSITIONS, pos = wave % C::POSITIONS;
+    const unsigned wm = (pos / (C::BT / C::WN)) * C::WM, wn = (pos % (C::BT / C::WN)) * C::WN;
     v16f acc[C::TM][C::TN];
 #pragma unroll
     for (int a = 0; a < C::TM; ++a)
@@ -287,18 +333,19 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
         for (int b = 0; b < C::TN; ++b)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.0f;
-    auto multiply = [&](const char* buf) {
+    const unsigned frag = (lane & 31) * 64, turn = lane >> 2 & 3, unit = (lane >> 5) * 2;
+    auto multiply = [&](const char* stage) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
+        for (int f = 0; f < C::F / C::KG; ++f) {
+            const char* buf = stage + (f * C::KG + group) * C::SLAB;
             h8 fp[C::TM][2], fq[C::TN][2];
-            const unsigned unit = (kk * 2 + (lane >> 5)) * 2, r = lane & 31;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const unsigned at = r * 128 + (((unit + h) ^ (r & 7)) * 16);
+                const unsigned at = frag + (((unit + h) ^ turn) * 16);
 #pragma unroll
-                for (int a = 0; a < C::TM; ++a) fp[a][h] = *reinterpret_cast<const h8*>(buf + (wm + a * 32) * 128 + at);
+                for (int a = 0; a < C::TM; ++a) fp[a][h] = *reinterpret_cast<const h8*>(buf + (wm + a * 32) * 64 + at);
 #pragma unroll
-                for (int b = 0; b < C::TN; ++b) fq[b][h] = *reinterpret_cast<const h8*>(buf + (C::BT + wn + b * 32) * 128 + at);
+                for (int b = 0; b < C::TN; ++b) fq[b][h] = *reinterpret_cast<const h8*>(buf + (C::BT + wn + b * 32) * 64 + at);
             }
 #pragma unroll
             for (int a = 0; a < C::TM; ++a)
@@ -310,15 +357,119 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
                 }
         }
     };
-    const unsigned steps = k / 32;                   // even: k is a multiple of 64
-    load(s_buf0, 0);
+    // Waits until at most `in_flight` stages of this wave's loads are on their way (they land in order), then
+    // for the other waves to have got there: the stage that is multiplied next is in LDS, and every wave is
+    // done with the one before, whose buffer the next load overwrites.
+    auto arrive = [&](auto in_flight) {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        constexpr int n = decltype(in_flight)::value * C::LOADS;
+        __builtin_amdgcn_s_waitcnt((n & 15) | ((n >> 4) << 14) | 0x0F70);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    constexpr unsigned kAhead = C::RING - 1;         // stages on their way when one is multiplied
+    typedef std::integral_constant<int, int(kAhead) - 1> Full;
+    typedef std::integral_constant<int, 1> One;
+    typedef std::integral_constant<int, 0> None;
+    const unsigned stages = k / (16 * C::F);         // k is a multiple of 64, F of 1, 2 or 4
+    // one stage: how many later ones have been asked for decides the wait
+    auto turn_of = [&](const char* now, char* next, unsigned s) {
+        const unsigned later = stages - 1 - s;
+        if (later >= kAhead - 1) arrive(Full{});
+        else if (later == 1) arrive(One{});
+        else arrive(None{});
+        if (later >= kAhead) load(next, s + kAhead);
+        multiply(now);
+    };
+    load(s_ring0, 0);
+    if (stages > 1) load(s_ring1, 1);
+    if (C::RING == 4 && stages > 2) load(s_ring2, 2);
+    if (C::RING == 4) {
+        unsigned s = 0;
+        for (; s + 7 <= stages; s += 4) {            // s + 6 is the last stage that this turn asks for
+            arrive(Full{});
+            load(s_ring3, s + 3);
+            multiply(s_ring0);
+            arrive(Full{});
+            load(s_ring0, s + 4);
+            multiply(s_ring1);
+            arrive(Full{});
+            load(s_ring1, s + 5);
+            multiply(s_ring2);
+            arrive(Full{});
+            load(s_ring2, s + 6);
+            multiply(s_ring3);
+        }
+        for (; s < stages; s += 4) {
+            turn_of(s_ring0, s_ring3, s);
+            if (s + 1 < stages) turn_of(s_ring1, s_ring0, s + 1);
+            if (s + 2 < stages) turn_of(s_ring2, s_ring1, s + 2);
+            if (s + 3 < stages) turn_of(s_ring3, s_ring2, s + 3);
+        }
+    } else {
+        unsigned s = 0;
+        for (; s + 5 <= stages; s += 3) {
+            arrive(Full{});
+            load(s_ring2, s + 2);
+            multiply(s_ring0);
+            arrive(Full{});
+            load(s_ring0, s + 3);
+            multiply(s_ring1);
+            arrive(Full{});
+            load(s_ring1, s + 4);
+            multiply(s_ring2);
+        }
+        for (; s < stages; s += 3) {
+            turn_of(s_ring0, s_ring2, s);
+            if (s + 1 < stages) turn_of(s_ring1, s_ring0, s + 1);
+            if (s + 2 < stages) turn_of(s_ring2, s_ring1, s + 2);
+        }
+    }
     __syncthreads();
-    for (unsigned s = 0; s < steps; s += 2) {
-        load(s_buf1, s + 1);
-        multiply(s_buf0);
+    // 4 KiB pieces of the ring
+    constexpr unsigned kPieces = C::STAGE / 4096;
+    auto piece = [&](unsigned i) {
+        const unsigned ring = i / kPieces;
+        return (ring == 0 ? s_ring0 : ring == 1 ? s_ring1 : ring == 2 ? s_ring2 : s_ring3) + (i % kPieces) * 4096;
+    };
+    // The groups of a position add their sums: tile t of the wave's goes to group t % KG, in group order.
+    auto mine = [&](int tile) { return C::KG == 1 || unsigned(tile) % C::KG == group; };
+    if (C::KG > 1) {
+        constexpr int kTiles = C::TM * C::TN;
+#pragma unroll
+        for (int a = 0; a < C::TM; ++a)
+#pragma unroll
+            for (int b = 0; b < C::TN; ++b) {
+                const int tile = a * C::TN + b;
+                if (mine(tile)) continue;
+                const unsigned rank = group < unsigned(tile) % C::KG ? group : group - 1;
+                v4f* dst = reinterpret_cast<v4f*>(piece((rank * C::POSITIONS + pos) * kTiles + tile)) + lane;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const v4f v = {acc[a][b][4 * e], acc[a][b][4 * e + 1], acc[a][b][4 * e + 2], acc[a][b][4 * e + 3]};
+                    dst[e * 64] = v;
+                }
+            }
         __syncthreads();
-        if (s + 2 < steps) load(s_buf0, s + 2);
-        multiply(s_buf1);
+#pragma unroll
+        for (int a = 0; a < C::TM; ++a)
+#pragma unroll
+            for (int b = 0; b < C::TN; ++b) {
+                const int tile = a * C::TN + b;
+                if (!mine(tile)) continue;
+#pragma unroll
+                for (unsigned rank = 0; rank < C::KG - 1; ++rank) {
+                    const v4f* src = reinterpret_cast<const v4f*>(piece((rank * C::POSITIONS + pos) * kTiles + tile)) + lane;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const v4f v = src[e * 64];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) acc[a][b][4 * e + x] += v[x];
+                    }
+                }
+            }
         __syncthreads();
     }
 
@@ -328,14 +479,14 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
     char* direct = KIND == GRAM ? buf_a(j, work) : KIND == POLY ? buf_b(j, work) : buf_x(j, work, from ^ 1);
     char* turned = KIND == GRAM ? buf_a(j, work) : KIND == POLY ? buf_b(j, work) : buf_y(j, work, from ^ 1);
     const char* addend = KIND == POLY ? buf_a(j, work) : buf_y(j, work, from);
-    uint32_t* s_turn = reinterpret_cast<uint32_t*>(s_buf0) + wave * 1024;
+    uint32_t* s_turn = reinterpret_cast<uint32_t*>(piece(wave));       // a 32 x 32 tile per wave is turned in LDS
     const unsigned half = lane >> 5, col = lane & 31;
 #pragma unroll
     for (int a = 0; a < C::TM; ++a)
 #pragma unroll
         for (int b = 0; b < C::TN; ++b) {
             const unsigned gi = i0 + wm + a * 32, gj = j0 + wn + b * 32;
-            if (gi >= rows_p || gj >= rows_q) continue;                        // wave-uniform; rows are multiples of 64
+            if (!mine(a * C::TN + b) || gi >= rows_p || gj >= rows_q) continue;     // wave-uniform; rows are multiples of 64
 #pragma unroll
             for (int quad = 0; quad < 4; ++quad) {
                 const size_t at = (size_t(gj + col) * ld_turned + gi) * 4 + quad * 32 + half * 8;
@@ -404,6 +555,436 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
         }
 }
 
+// ------------------------------------------------------------------------------- narrow matrices
+// m <= 64: B is one or four tiles of 32 x 32, and a wave that owns 32 columns of X needs nothing of the
+// other columns but their share of X X^T.  The layout in which an MFMA leaves its sums - column in the lane,
+// rows in the registers - is one in which the next MFMA can take them, as long as both operands run
+// through the contracted rows in that order: X enters B X as it stands, and so do the symmetric A and B, which
+// are their own transposes.  Only X X^T contracts over the lanes; there the tile is turned by a product with
+// the identity, exact in fp32.  So X stays in registers through all steps, in fp32 (times 2^13), and LDS
+// carries nothing but the waves' shares of X X^T and, with four tiles, of A A.  The two low halves' product
+// is included: it costs nothing here.
+// A matrix of one stripe (a block's columns) goes through all its steps in one launch; with more stripes, a
+// launch per step: every block adds the stripes' shares for itself, in order.
+enum NarrowMode { WHOLE, FIRST, NEXT };
+constexpr unsigned kTileFloats = 1024;
+
+struct Pairs {                                        // an operand of 32 contracted rows: two MFMA steps
+    h8 hi[2], lo[2];
+};
+__device__ __forceinline__ Pairs pairs_of(const float (&v)[16]) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    Pairs r;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const v2f x = {v[8 * s + e], v[8 * s + e + 1]};
+            const h2 h = __builtin_convertvector(x, h2);
+            const v2f d = {x[0] - float(h[0]), x[1] - float(h[1])};
+            const h2 l = __builtin_convertvector(d, h2);
+            r.hi[s][e] = h[0];
+            r.hi[s][e + 1] = h[1];
+            r.lo[s][e] = l[0];
+            r.lo[s][e + 1] = l[1];
+        }
+    return r;
+}
+__device__ __forceinline__ void multiply_pairs(v16f& acc, const Pairs& p, const Pairs& q) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p.lo[s], q.lo[s], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p.hi[s], q.lo[s], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p.lo[s], q.hi[s], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p.hi[s], q.hi[s], acc, 0, 0, 0);
+    }
+}
+__device__ __forceinline__ v16f zero16() {
+    v16f z;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) z[e] = 0.0f;
+    return z;
+}
+// a tile of 32 x 32 floats in memory: [register / 4][lane][register % 4]
+__device__ __forceinline__ void put_tile(float* to, unsigned lane, const float (&v)[16]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const v4f w = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+        *reinterpret_cast<v4f*>(to + (q * 64 + lane) * 4) = w;
+    }
+}
+__device__ __forceinline__ void add_tile(const float* from, unsigned lane, float (&v)[16]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const v4f w = *reinterpret_cast<const v4f*>(from + (q * 64 + lane) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * q + e] += w[e];
+    }
+}
+
+// ROWS: tiles of rows, 1 or 2.  WAVES: waves of a block, 32 columns each.
+template <int ROWS_, int WAVES_>
+struct NarrowCfg {
+    static constexpr int ROWS = ROWS_, WAVES = WAVES_, STRIPE = 32 * WAVES_, TILES = ROWS * ROWS, THREADS = 64 * WAVES_;
+    // ROWS == 1: the waves' shares twice (a wave may be a step ahead of another that still reads).
+    // ROWS == 2: the shares - and in their place, later in a step, the parts of A A - and their sum.
+    static constexpr int SHARES = ROWS == 1 ? 2 * WAVES : WAVES * TILES;
+    static_assert(STRIPE * (32 * ROWS + 1) <= SHARES * int(kTileFloats), "a tall matrix's stripe is turned in the shares' place");
+};
+typedef NarrowCfg<1, 8> Flat;                         // up to 32 x 256
+typedef NarrowCfg<1, 16> FlatWide;                    // up to 32 x 512
+typedef NarrowCfg<2, 8> Narrow;                       // up to 64 x 256
+
+__host__ __device__ inline unsigned stripes_of(const Job& j, int stripe) { return unsigned(j.n + stripe - 1) / unsigned(stripe); }
+// workspace of a matrix of several stripes: the norm's parts, the stripes' tiles of X, their shares of X X^T
+// twice (a block may be a step ahead of another that still reads); sized for the narrowest stripe
+constexpr int kLeastStripe = 256;
+__host__ __device__ inline size_t narrow_floats(const Job& j) { return size_t(stripes_of(j, kLeastStripe)) * (kLeastStripe * 64 + 2 * 4 * kTileFloats); }
+__device__ inline float* narrow_x(char* w) { return reinterpret_cast<float*>(w + kNormBytes); }
+__device__ inline float* narrow_shares(const Job& j, char* w, int which) {
+    return narrow_x(w) + size_t(stripes_of(j, kLeastStripe)) * (kLeastStripe * 64 + size_t(which) * 4 * kTileFloats);
+}
+
+__device__ inline unsigned left_of(const Job& j, unsigned stripe, unsigned wide) {
+    const unsigned left = unsigned(j.n) - stripe * wide;
+    return left < wide ? left : wide;
+}
+
+// MODE WHOLE: momentum, norm and all steps.  FIRST: the normalised stripe and its share of the first X X^T.
+// NEXT: one step; `last` writes the result.
+template <NarrowMode MODE, class C>
+__global__ __launch_bounds__(C::THREADS) void narrow_product(Table t, int steps, int parity, int last, float ca, float cb, float cc) {
+    constexpr int ROWS = C::ROWS, TILES = C::TILES, WAVES = C::WAVES;
+    __shared__ __attribute__((aligned(16))) float s_share[C::SHARES * kTileFloats];
+    __shared__ __attribute__((aligned(16))) float s_sum[TILES * kTileFloats];
+    __shared__ double s_part[WAVES];
+    const int which = job_of(t, blockIdx.x);
+    const Job& j = t.job[which];
+    const unsigned local = blockIdx.x - t.first[which], stripes = stripes_of(j, C::STRIPE), item = local / stripes, stripe = local % stripes;
+    char* work = j.work + item * j.work_stride;
+    const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
+    const unsigned j0 = stripe * C::STRIPE + wave * 32, gj = j0 + (lane & 31);
+    const bool live = j0 < unsigned(j.n);                                          // wave-uniform
+    // register e of tile a is element (32 a + 8 (e / 4) + 4 half + e % 4, gj).  Loads go to a place inside the
+    // matrix whatever the register (no branch, all of them on their way at once); 2^20 x 64 has 32-bit places.
+    const size_t matrix = item * j.stride;
+    const unsigned cols = unsigned(j.cols), down = j.tall ? 1 : cols, across = j.tall ? cols : 1, last_row = unsigned(j.m) - 1;
+    const bool in_col = gj < unsigned(j.n);
+    unsigned corner = (in_col ? gj : unsigned(j.n) - 1) * across;
+    auto row_of = [&](int a, int e) { return unsigned(a) * 32 + unsigned(e >> 2) * 8 + half * 4 + unsigned(e & 3); };
+    auto inside = [&](int a, int e) { return in_col && row_of(a, e) <= last_row; };
+    auto address = [&](int a, int e) {
+        const unsigned r = row_of(a, e);
+        return corner + (r < last_row ? r : last_row) * down;
+    };
+    auto fetch = [&](const float* from, int a, float (&v)[16]) {
+        from += matrix;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = from[address(a, e)];
+    };
+    // The stripe of a tall matrix is one run of memory, m values to a column of X: it is walked in that order
+    // and changes its layout in LDS (columns an odd number of words apart).  every(place, place in LDS)
+    const unsigned pitch = unsigned(j.m) | 1, run = (left_of(j, stripe, C::STRIPE)) * unsigned(j.m);
+    const size_t run0 = matrix + size_t(stripe) * C::STRIPE * unsigned(j.m);
+    auto walk = [&](auto every) {
+        const unsigned m = unsigned(j.m), step_col = C::THREADS / m, step_row = C::THREADS % m;
+        unsigned c = threadIdx.x / m, r = threadIdx.x % m;
+#pragma unroll 4
+        for (unsigned i = threadIdx.x; i < run; i += C::THREADS) {
+            every(run0 + i, c * pitch + r);
+            c += step_col;
+            r += step_row;
+            if (r >= m) {
+                r -= m;
+                ++c;
+            }
+        }
+    };
+    auto at_pitch = [&](int a, int e) { return (wave * 32 + (lane & 31)) * pitch + row_of(a, e); };
+    auto block_total = [&](double v) {
+        for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+        if (lane == 0) s_part[wave] = v;
+        __syncthreads();
+        v = 0.0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) v += s_part[w];
+        return 1.0 / (sqrt(v) + double(t.eps));
+    };
+
+    float x[ROWS][16];
+#pragma unroll
+    for (int a = 0; a < ROWS; ++a)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[a][e] = 0.0f;
+    float* x_tiles = narrow_x(work) + (size_t(stripe) * WAVES + wave) * ROWS * kTileFloats;
+    if (MODE == NEXT) {
+        if (live)
+#pragma unroll
+            for (int a = 0; a < ROWS; ++a) add_tile(x_tiles + a * kTileFloats, lane, x[a]);
+    } else {
+        double sum = 0.0;
+        if (j.tall) {
+            walk([&](size_t at, unsigned to) {
+                float u;
+                if (MODE == WHOLE) {
+                    u = j.grad[at];
+                    if (j.momentum) {
+                        const float v = t.mu * j.momentum[at] + u;
+                        j.new_momentum[at] = v;
+                        u = t.nesterov ? u + t.mu * v : v;
+                    }
+                    sum += double(u) * double(u);
+                } else {
+                    u = update_at(t, j, at);
+                }
+                s_share[to] = u;
+            });
+            if (MODE == FIRST)
+                for (unsigned i = threadIdx.x; i < j.norm_parts; i += C::THREADS) sum += reinterpret_cast<const double*>(work)[i];
+        } else if (MODE == WHOLE) {
+#pragma unroll
+            for (int a = 0; a < ROWS; ++a) fetch(j.grad, a, x[a]);
+            if (j.momentum) {
+                float m[ROWS][16];
+#pragma unroll
+                for (int a = 0; a < ROWS; ++a) fetch(j.momentum, a, m[a]);
+#pragma unroll
+                for (int a = 0; a < ROWS; ++a)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float v = t.mu * m[a][e] + x[a][e];
+                        if (inside(a, e)) j.new_momentum[matrix + address(a, e)] = v;
+                        x[a][e] = t.nesterov ? x[a][e] + t.mu * v : v;
+                    }
+            }
+#pragma unroll
+            for (int a = 0; a < ROWS; ++a)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sum += inside(a, e) ? double(x[a][e]) * double(x[a][e]) : 0.0;
+        } else {
+            for (unsigned i = threadIdx.x; i < j.norm_parts; i += C::THREADS) sum += reinterpret_cast<const double*>(work)[i];
+#pragma unroll
+            for (int a = 0; a < ROWS; ++a) fetch(j.momentum && !t.nesterov ? j.new_momentum : j.grad, a, x[a]);
+            if (j.momentum && t.nesterov) {
+                float m[ROWS][16];
+#pragma unroll
+                for (int a = 0; a < ROWS; ++a) fetch(j.new_momentum, a, m[a]);
+#pragma unroll
+                for (int a = 0; a < ROWS; ++a)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[a][e] = x[a][e] + t.mu * m[a][e];
+            }
+        }
+        const double inv = block_total(sum);          // a barrier: the run is in LDS
+        if (j.tall)
+#pragma unroll
+            for (int a = 0; a < ROWS; ++a)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (inside(a, e)) x[a][e] = s_share[at_pitch(a, e)];
+        if (j.tall) __syncthreads();                  // the shares overwrite it
+#pragma unroll
+        for (int a = 0; a < ROWS; ++a)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[a][e] = inside(a, e) ? float(x[a][e] * inv) * kScaleX : 0.0f;     // inf * 0 is no zero
+    }
+    // the identity as the second operand, in the order of the contracted rows
+    h8 eye[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) eye[s][e] = row_of(0, 8 * s + e) == (lane & 31) ? _Float16(1) : _Float16(0);
+
+    Pairs xp[ROWS];
+    auto pair_x = [&]() {
+#pragma unroll
+        for (int a = 0; a < ROWS; ++a) xp[a] = pairs_of(x[a]);
+    };
+    // this wave's share of X X^T to LDS, from the turned tiles
+    auto put_shares = [&](float* shares) {
+        Pairs xt[ROWS];
+#pragma unroll
+        for (int a = 0; a < ROWS; ++a) {
+            v16f acc = zero16();
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(xp[a].hi[s], eye[s], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(xp[a].lo[s], eye[s], acc, 0, 0, 0);
+            }
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = acc[e];
+            xt[a] = pairs_of(v);
+        }
+#pragma unroll
+        for (int a = 0; a < ROWS; ++a)
+#pragma unroll
+            for (int b = 0; b < ROWS; ++b) {
+                v16f acc = zero16();
+                multiply_pairs(acc, xt[a], xt[b]);
+                float v[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = acc[e] * (1.0f / (kScaleX * kScaleX));
+                put_tile(shares + (wave * TILES + a * ROWS + b) * kTileFloats, lane, v);
+            }
+    };
+    // The sum of the waves' shares.  One tile: every wave adds them for itself.  Four: a thread adds its
+    // eight elements, into s_sum.
+    auto own_sum = [&](const float* shares, float (&v)[16]) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) add_tile(shares + w * kTileFloats, lane, v);
+    };
+    constexpr unsigned kPerThread = TILES * kTileFloats / C::THREADS / 4;          // vectors of 4 (ROWS == 2)
+    auto joint_sum = [&](const float* shares, unsigned count, size_t stride, unsigned i) {
+        v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (unsigned w0 = 0; w0 < count; w0 += 8) {  // eight on their way at once; beyond the last, the last again
+            v4f r[8];
+#pragma unroll
+            for (unsigned w = 0; w < 8; ++w) r[w] = *reinterpret_cast<const v4f*>(shares + (w0 + w < count ? w0 + w : count - 1) * stride + size_t(i) * 4);
+#pragma unroll
+            for (unsigned w = 0; w < 8; ++w)
+                if (w0 + w < count) v += r[w];
+        }
+        return v;
+    };
+    // B from A (a: its one tile; four tiles are in s_sum), then X = ca X + B X
+    auto step = [&](const float (&a)[16]) {
+        if (ROWS == 1) {
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = a[e] * kScaleA;
+            const Pairs ap = pairs_of(v);
+            v16f acc = zero16();
+            multiply_pairs(acc, ap, ap);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = (cb * a[e] + acc[e] * (cc / (kScaleA * kScaleA))) * kScaleA;
+            const Pairs bp = pairs_of(v);
+            acc = zero16();
+            multiply_pairs(acc, bp, xp[0]);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[0][e] = ca * x[0][e] + acc[e] * (1.0f / kScaleA);
+            return;
+        }
+        // wave w forms the part of tile w % 4 of B that contracts over the rows of tile w / 4: (k, a) holds
+        // A[k][a] with a in the lane, which is A[a][k], the first operand of tile (a, b); (k, b) the second
+        {
+            const unsigned ta = wave >> 1 & 1, tb = wave & 1, tk = wave >> 2;
+            float p[16], q[16], v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) p[e] = q[e] = v[e] = 0.0f;
+            add_tile(s_sum + (tk * 2 + ta) * kTileFloats, lane, p);
+            add_tile(s_sum + (tk * 2 + tb) * kTileFloats, lane, q);
+            if (tk == 0) add_tile(s_sum + (ta * 2 + tb) * kTileFloats, lane, v);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                p[e] *= kScaleA;
+                q[e] *= kScaleA;
+            }
+            v16f acc = zero16();
+            multiply_pairs(acc, pairs_of(p), pairs_of(q));
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = (cb * v[e] + acc[e] * (cc / (kScaleA * kScaleA))) * kScaleA;
+            put_tile(s_share + wave * kTileFloats, lane, v);
+        }
+        __syncthreads();
+        Pairs bp[TILES];
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = 0.0f;
+            add_tile(s_share + i * kTileFloats, lane, v);
+            add_tile(s_share + (4 + i) * kTileFloats, lane, v);
+            bp[i] = pairs_of(v);
+        }
+        __syncthreads();                              // the next shares overwrite the parts
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            v16f acc = zero16();
+#pragma unroll
+            for (int k = 0; k < ROWS; ++k) multiply_pairs(acc, bp[k * ROWS + r], xp[k]);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[r][e] = ca * x[r][e] + acc[e] * (1.0f / kScaleA);
+        }
+    };
+    float a[16];
+    if (MODE == WHOLE) {
+#pragma unroll 1
+        for (int s = 0; s < steps; ++s) {
+            pair_x();
+            float* shares = s_share + (ROWS == 1 ? (s & 1) * WAVES * int(kTileFloats) : 0);
+            put_shares(shares);
+            __syncthreads();
+            if (ROWS == 1) {
+                own_sum(shares, a);
+            } else {
+#pragma unroll
+                for (unsigned i = 0; i < kPerThread; ++i)
+                    *reinterpret_cast<v4f*>(s_sum + (threadIdx.x + i * C::THREADS) * 4) =
+                        joint_sum(shares, WAVES, TILES * kTileFloats, threadIdx.x + i * C::THREADS);
+                __syncthreads();
+            }
+            step(a);
+        }
+        asm volatile("" : "+v"(corner));              // the addresses are formed again, not kept through the steps
+    } else {
+        if (MODE == NEXT) {
+            const float* from = narrow_shares(j, work, parity);
+            for (unsigned i = threadIdx.x; i < TILES * kTileFloats / 4; i += C::THREADS)
+                *reinterpret_cast<v4f*>(s_sum + i * 4) = joint_sum(from, stripes, TILES * kTileFloats, i);
+            pair_x();
+            __syncthreads();
+            if (ROWS == 1) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) a[e] = 0.0f;
+                add_tile(s_sum, lane, a);
+            }
+            step(a);
+        }
+        if (!last) {
+            pair_x();
+            put_shares(s_share);
+            if (live)
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) put_tile(x_tiles + r * kTileFloats, lane, x[r]);
+            __syncthreads();
+            float* to = narrow_shares(j, work, MODE == FIRST ? 0 : parity ^ 1) + size_t(stripe) * TILES * kTileFloats;
+            for (unsigned i = threadIdx.x; i < TILES * kTileFloats / 4; i += C::THREADS)
+                *reinterpret_cast<v4f*>(to + i * 4) = joint_sum(s_share, WAVES, TILES * kTileFloats, i);
+        }
+    }
+    if (MODE == WHOLE || last) {
+        if (j.tall) {
+            __syncthreads();                          // everyone is done with what LDS holds
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (inside(r, e)) s_share[at_pitch(r, e)] = x[r][e] * (1.0f / kScaleX);
+            __syncthreads();
+            walk([&](size_t at, unsigned from) { j.out[at] = result_at(t, j, at, s_share[from]); });
+        } else if (j.param) {
+            float p[ROWS][16];
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) fetch(j.param, r, p[r]);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (inside(r, e)) j.out[matrix + address(r, e)] = p[r][e] * t.decay - j.step * (x[r][e] * (1.0f / kScaleX));
+        } else {
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (inside(r, e)) j.out[matrix + address(r, e)] = x[r][e] * (1.0f / kScaleX);
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------- host side
 constexpr int64_t kMostExtent = int64_t(1) << 20, kMostSide = int64_t(1) << 15;
 constexpr int kMostSteps = 64;
@@ -434,15 +1015,18 @@ void shape_job(Job* j, int64_t rows, int64_t cols, unsigned count) {
     j->count = count;
     j->stride = size_t(rows) * size_t(cols);
     size_t size = (j->stride + kNormParts - 1) / kNormParts;
-    if (size < 4096) size = 4096;
+    size = (size + 4095) / 4096 * 4096;
     j->part_size = size;
     j->norm_parts = unsigned((j->stride + size - 1) / size);
     j->work_stride = kNormBytes + 4 * pairs_xy(*j) + 2 * pairs_a(*j);
+    const size_t narrow = kNormBytes + narrow_floats(*j) * sizeof(float);
+    if (j->m <= 64 && narrow > j->work_stride) j->work_stride = narrow;
 }
 
-typedef TileCfg<64, 32, 32> Tile64;
-typedef TileCfg<128, 64, 64> Tile128;
-typedef TileCfg<256, 128, 64> Tile256;
+typedef TileCfg<64, 32, 32, 4, 4, 4> Tile64;
+typedef TileCfg<128, 64, 64, 2, 2, 4> Tile128;
+typedef TileCfg<192, 96, 96, 2, 2, 3> Tile192;
+typedef TileCfg<256, 128, 64, 1, 1, 4> Tile256;
 
 double flops_of(const Job& j, int steps) {
     const double m = j.m, n = j.n;
@@ -457,33 +1041,99 @@ unsigned lay_out(Table* t, F per) {
     return t->first[t->jobs];
 }
 
-template <class C>
+unsigned sym_tiles(const Job& j, unsigned bt) {
+    const unsigned tm = (unsigned(j.mp) + bt - 1) / bt;
+    return tm * (tm + 1) / 2;
+}
+unsigned full_tiles(const Job& j, unsigned bt) { return ((unsigned(j.mp) + bt - 1) / bt) * ((unsigned(j.np) + bt - 1) / bt); }
+
+// The tile of a launch: the one whose rounds of one block per CU cost least.
+template <class F>
+int pick_tile(const Table& t, F tiles) {
+    const size_t cus = size_t(compute_units() > 0 ? compute_units() : 256);
+    const int sizes[4] = {256, 192, 128, 64};
+    const double cost[4] = {16.0, 9.6, 5.0, 1.9};
+    int best = 256;
+    double least = 1e300;
+    for (int i = 0; i < 4; ++i) {
+        size_t blocks = 0;
+        for (int j = 0; j < t.jobs; ++j) blocks += size_t(t.job[j].count) * tiles(t.job[j], unsigned(sizes[i]));
+        const double c = double((blocks + cus - 1) / cus) * cost[i];
+        if (c < least) {
+            least = c;
+            best = sizes[i];
+        }
+    }
+    return best;
+}
+
+template <class C, Kind KIND>
+void launch_product(Table* t, int from, const float* c, hipStream_t s) {
+    const unsigned blocks = lay_out(t, [](const Job& j) { return KIND == GRAM || KIND == POLY ? sym_tiles(j, C::BT) : full_tiles(j, C::BT); });
+    hipLaunchKernelGGL((pair_product<C, KIND>), dim3(blocks), dim3(C::THREADS), 0, s, *t, from, c[0], c[1], c[2]);
+}
+template <Kind KIND>
+void launch_product(int tile, Table* t, int from, const float* c, hipStream_t s) {
+    if (tile == 256) launch_product<Tile256, KIND>(t, from, c, s);
+    else if (tile == 192) launch_product<Tile192, KIND>(t, from, c, s);
+    else if (tile == 128) launch_product<Tile128, KIND>(t, from, c, s);
+    else launch_product<Tile64, KIND>(t, from, c, s);
+}
+
 int iterate(const char* who, Table* t, int steps, const float* c, hipStream_t s) {
-    auto sym = [](const Job& j) {
-        const unsigned tm = (unsigned(j.mp) + C::BT - 1) / C::BT;
-        return tm * (tm + 1) / 2;
-    };
-    auto full = [](const Job& j) { return ((unsigned(j.mp) + C::BT - 1) / C::BT) * ((unsigned(j.np) + C::BT - 1) / C::BT); };
+    const int sym = pick_tile(*t, sym_tiles), full = pick_tile(*t, full_tiles);
     for (int k = 0; k < steps; ++k) {
         const int from = k & 1;
-        unsigned blocks = lay_out(t, sym);
-        hipLaunchKernelGGL((pair_product<C, GRAM>), dim3(blocks), dim3(C::THREADS), 0, s, *t, from, c[0], c[1], c[2]);
-        hipLaunchKernelGGL((pair_product<C, POLY>), dim3(blocks), dim3(C::THREADS), 0, s, *t, from, c[0], c[1], c[2]);
-        blocks = lay_out(t, full);
-        if (k + 1 < steps) hipLaunchKernelGGL((pair_product<C, STEP>), dim3(blocks), dim3(C::THREADS), 0, s, *t, from, c[0], c[1], c[2]);
-        else hipLaunchKernelGGL((pair_product<C, LAST>), dim3(blocks), dim3(C::THREADS), 0, s, *t, from, c[0], c[1], c[2]);
+        launch_product<GRAM>(sym, t, from, c, s);
+        launch_product<POLY>(sym, t, from, c, s);
+        if (k + 1 < steps) launch_product<STEP>(full, t, from, c, s);
+        else launch_product<LAST>(full, t, from, c, s);
         const int rc = launched(who);
         if (rc) return rc;
     }
     return CTAMD_OK;
 }
 
+// Whether the narrow kernels take a matrix: beyond some stripes the blocks' sums of all shares cost more than
+// the separate products' launches.
+constexpr unsigned kMostStripes = 32;
+bool is_narrow(const Job& j) { return j.m <= 64 && stripes_of(j, kLeastStripe) <= kMostStripes; }
+
+template <class C>
+void launch_whole(Table* t, int steps, const float* c, hipStream_t s) {
+    const unsigned blocks = lay_out(t, [](const Job&) { return 1u; });
+    hipLaunchKernelGGL((narrow_product<WHOLE, C>), dim3(blocks), dim3(C::THREADS), 0, s, *t, steps, 0, 1, c[0], c[1], c[2]);
+}
+template <class C>
+void iterate_narrow(Table* t, int steps, const float* c, hipStream_t s) {
+    const unsigned blocks = lay_out(t, [](const Job& j) { return stripes_of(j, C::STRIPE); });
+    hipLaunchKernelGGL((narrow_product<FIRST, C>), dim3(blocks), dim3(C::THREADS), 0, s, *t, 0, 0, 0, c[0], c[1], c[2]);
+    for (int k = 0; k < steps; ++k)
+        hipLaunchKernelGGL((narrow_product<NEXT, C>), dim3(blocks), dim3(C::THREADS), 0, s, *t, 0, k & 1, int(k + 1 == steps), c[0], c[1], c[2]);
+}
+
 int run_table(const char* who, Table* t, int steps, const float* c, hipStream_t s) {
     if (!t->jobs) return CTAMD_OK;
+    for (int k = 0; k < t->jobs; ++k) {
+        Job& j = t->job[k];
+        j.vec = j.cols % 4 == 0 && aligned16(j.grad) && (!j.momentum || (aligned16(j.momentum) && aligned16(j.new_momentum)));
+    }
     double bytes = 0, flops = 0;
+    bool narrow = true;
+    int most_m = 0, most_n = 0;
     for (int j = 0; j < t->jobs; ++j) {
+        narrow = narrow && is_narrow(t->job[j]);
+        if (t->job[j].m > most_m) most_m = t->job[j].m;
+        if (t->job[j].n > most_n) most_n = t->job[j].n;
         bytes += (t->job[j].param ? 20.0 : 8.0) * double(t->job[j].stride) * t->job[j].count;
         flops += flops_of(t->job[j], steps);
+    }
+    if (narrow && (most_m <= 32 ? most_n <= FlatWide::STRIPE : most_n <= Narrow::STRIPE)) {
+        if (most_m > 32) launch_whole<Narrow>(t, steps, c, s);
+        else if (most_n > Flat::STRIPE) launch_whole<FlatWide>(t, steps, c, s);
+        else launch_whole<Flat>(t, steps, c, s);
+        account(bytes, flops);
+        return launched(who);
     }
     unsigned blocks = lay_out(t, [](const Job& j) { return j.norm_parts; });
     hipLaunchKernelGGL(momentum_norm, dim3(blocks), dim3(kThreads), 0, s, *t);
@@ -492,20 +1142,16 @@ int run_table(const char* who, Table* t, int steps, const float* c, hipStream_t 
     if (steps == 0) {
         hipLaunchKernelGGL(scaled_update, dim3(blocks), dim3(kThreads), 0, s, *t);
         rc = launched(who);
+    } else if (narrow) {
+        if (most_m <= 32) iterate_narrow<FlatWide>(t, steps, c, s);
+        else iterate_narrow<Narrow>(t, steps, c, s);
+        rc = launched(who);
     } else {
         blocks = lay_out(t, [](const Job& j) { return unsigned(j.mp / 64) * unsigned(j.np / 64); });
         hipLaunchKernelGGL(load_pairs, dim3(blocks), dim3(kThreads), 0, s, *t);
         rc = launched(who);
         if (rc) return rc;
-        const size_t cus = size_t(compute_units() > 0 ? compute_units() : 256);
-        size_t at256 = 0, at128 = 0;
-        for (int j = 0; j < t->jobs; ++j) {
-            const Job& b = t->job[j];
-            at256 += size_t(b.count) * ((b.mp + 255) / 256) * ((b.np + 255) / 256);
-            at128 += size_t(b.count) * ((b.mp + 127) / 128) * ((b.np + 127) / 128);
-        }
-        rc = at256 >= cus * 3 / 4 ? iterate<Tile256>(who, t, steps, c, s)
-             : at128 >= cus * 3 / 4 ? iterate<Tile128>(who, t, steps, c, s) : iterate<Tile64>(who, t, steps, c, s);
+        rc = iterate(who, t, steps, c, s);
     }
     if (!rc) account(bytes, flops);
     return rc;
