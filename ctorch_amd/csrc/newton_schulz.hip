@@ -12,11 +12,13 @@
 // iteration ends where the one in fp32 products does (2.4e-6 of the largest entry for both at 1024 x 1024):
 // the polynomial's slope at zero, a^steps, magnifies any rounding of the first steps alike.
 //
-// Layout of a matrix of pairs: row-major, rows padded to 64 columns (zeros), each run of 8 columns stored as
-// [8 hi][8 lo], 32 bytes.  A k step of 16 is 64 bytes of a row and goes to LDS by the direct-to-LDS load;
-// 16-byte units are permuted by bits 2 and 3 of the row, so that the 16 lanes that the 64 banks serve at
-// once (of a ds_read_b128 per 32 x 16 operand half) meet no bank twice.  Both operands of every product are read
-// along their rows (A and B are symmetric; X is kept with its transpose Y), so one kernel serves all three.
+// Layout of a matrix of pairs: padded to 64 rows and columns (zeros), in panels of 16 columns, a panel row by
+// row: [8 hi][8 lo][8 hi][8 lo], 64 bytes.  A k step of a tile is then one run of memory per operand, which
+// the direct-to-LDS loads take in whole cache lines (rows of 64 bytes at a row's distance gave half the
+// bandwidth: 65 against 130 GB/s per CU).  The 16-byte units of a row are permuted by bits 2 and 3 of
+// its number, so that the 16 lanes that the 64 banks serve at once (of a ds_read_b128 per 32 x 16 operand
+// half) meet no bank twice.  Both operands of every product are read along their rows (A and B are symmetric;
+// X is kept with its transpose Y), so one kernel serves all three.
 #include <cmath>
 #include <type_traits>
 
@@ -156,6 +158,11 @@ __device__ __forceinline__ void split8(const float (&v)[8], float scale, h8* hi,
     }
 }
 
+// byte place of the 8 columns from k on of a row, in a matrix of `rows` padded rows
+__device__ __forceinline__ size_t pair_at(unsigned rows, unsigned row, unsigned k) {
+    return (size_t(k >> 4) * rows + row) * 64 + (k >> 3 & 1) * 32;
+}
+
 // Divides the update by its norm and writes it as pairs, straight and transposed; a block per 64 x 64 tile.
 __global__ __launch_bounds__(kThreads) void load_pairs(Table t) {
     __shared__ double s_part[kThreads / 64];
@@ -171,47 +178,40 @@ __global__ __launch_bounds__(kThreads) void load_pairs(Table t) {
     char* straight = j.tall ? buf_y(j, work, 0) : buf_x(j, work, 0);
     char* turned = j.tall ? buf_x(j, work, 0) : buf_y(j, work, 0);
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const unsigned r = (threadIdx.x >> 3) + 32 * q, c = (threadIdx.x & 7) * 8;
-        float v[8];
+    for (int q = 0; q < 4; ++q) {
+        const unsigned r = (threadIdx.x >> 4) + 16 * q, c = (threadIdx.x & 15) * 4;
         const size_t at = item * j.stride + size_t(r0 + r) * j.cols + c0 + c;
-        if (j.vec && int64_t(r0 + r) < j.rows && int64_t(c0 + c + 8) <= j.cols) {
+        float v[4];
+        if (j.vec && int64_t(r0 + r) < j.rows && int64_t(c0 + c) < j.cols) {
+            v4f u = *reinterpret_cast<const v4f*>((j.momentum && !t.nesterov ? j.new_momentum : j.grad) + at);
+            if (j.momentum && t.nesterov) {
+                const v4f m = *reinterpret_cast<const v4f*>(j.new_momentum + at);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                v4f u = *reinterpret_cast<const v4f*>((j.momentum && !t.nesterov ? j.new_momentum : j.grad) + at + 4 * h);
-                if (j.momentum && t.nesterov) {
-                    const v4f m = *reinterpret_cast<const v4f*>(j.new_momentum + at + 4 * h);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) u[e] = u[e] + t.mu * m[e];
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * h + e] = float(u[e] * inv);
+                for (int e = 0; e < 4; ++e) u[e] = u[e] + t.mu * m[e];
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = float(u[e] * inv);
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < 4; ++e) {
                 const bool in = int64_t(r0 + r) < j.rows && int64_t(c0 + c + e) < j.cols;
                 v[e] = in ? float(update_at(t, j, at + e) * inv) : 0.0f;
             }
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s_tile[r][c + e] = v[e];
-        h8 hi, lo;
-        split8(v, kScaleX, &hi, &lo);
-        h8* dst = reinterpret_cast<h8*>(straight + (size_t(r0 + r) * cp + c0 + c) * 4);
-        dst[0] = hi;
-        dst[1] = lo;
+        for (int e = 0; e < 4; ++e) s_tile[r][c + e] = v[e];
     }
     __syncthreads();
+    // 8 columns of a row to a thread: neighbouring threads fill neighbouring memory of a panel
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const unsigned c = (threadIdx.x >> 3) + 32 * q, r = (threadIdx.x & 7) * 8;
+    for (int q = 0; q < 4; ++q) {
+        const unsigned side = q >> 1, row = threadIdx.x >> 1 & 63, k = (threadIdx.x >> 7) * 16 + (q & 1) * 32 + (threadIdx.x & 1) * 8;
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = s_tile[r + e][c];
+        for (int e = 0; e < 8; ++e) v[e] = side == 0 ? s_tile[row][k + e] : s_tile[k + e][row];
         h8 hi, lo;
         split8(v, kScaleX, &hi, &lo);
-        h8* dst = reinterpret_cast<h8*>(turned + (size_t(c0 + c) * rp + r0 + r) * 4);
+        h8* dst = reinterpret_cast<h8*>(side == 0 ? straight + pair_at(rp, r0 + row, c0 + k) : turned + pair_at(cp, c0 + row, r0 + k));
         dst[0] = hi;
         dst[1] = lo;
     }
@@ -243,8 +243,7 @@ __global__ __launch_bounds__(kThreads) void scaled_update(Table t) {
 enum Kind { GRAM, POLY, STEP, LAST };
 
 // A block computes a BT x BT tile.  Its waves stand in (BT / WM) x (BT / WN) positions, KG waves to a
-// position, and those share the k range: a stage of the ring is F slabs of 16 k, wave group g multiplies
-// the slabs g, g + KG, ...  (a large wave tile reads each fragment from LDS for more MFMAs; on a small
+// position, and those share the k range: a stage of the ring is a slab of 16 k for each group (a large wave tile reads each fragment from LDS for more MFMAs; on a small
 // block tile only the k range is left to share).  RING stages, all but one on their way.
 template <int BT_, int WM_, int WN_, int KG_, int F_, int RING_>
 struct TileCfg {
@@ -255,7 +254,7 @@ struct TileCfg {
     static constexpr int SLAB = 2 * BT * 64, STAGE = F * SLAB; // bytes
     static constexpr int LOADS = F * UNITS / WAVES;            // loads per wave and stage
     static_assert(F * UNITS % WAVES == 0 && (UNITS % WAVES == 0 || WAVES % UNITS == 0), "the waves share a stage's loads evenly");
-    static_assert(F % KG == 0 && (RING == 3 || RING == 4), "");
+    static_assert(F == KG && (RING == 3 || RING == 4), "a slab of a stage to a group");
     static_assert(WAVES * 4096 <= RING * STAGE, "the epilogue turns a 32 x 32 tile per wave in the ring");
     static_assert((KG - 1) * BT * BT * 4 <= RING * STAGE, "the groups' sums meet in the ring");
 };
@@ -311,15 +310,16 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
         unsigned r = (second ? unit - kHalf : unit) * 16 + (lane >> 2);
         const unsigned most = (second ? rows_q - j0 : rows_p - i0) - 1;
         if (r > most) r = most;
-        off[l] = r * k * 4 + slab * 64 + ((lane & 3) ^ (lane >> 4 & 3)) * 16;
+        off[l] = (slab * (second ? rows_q : rows_p) + r) * 64 + ((lane & 3) ^ (lane >> 4 & 3)) * 16;
     }
-    const char* pb = p + size_t(i0) * k * 4;
-    const char* qb = q + size_t(j0) * k * 4;
+    const char* pb = p + size_t(i0) * 64;
+    const char* qb = q + size_t(j0) * 64;
+    const size_t stage_p = size_t(C::F) * rows_p * 64, stage_q = size_t(C::F) * rows_q * 64;
     auto load = [&](char* buf, unsigned stage) {
 #pragma unroll
         for (int l = 0; l < C::LOADS; ++l) {
             const unsigned u = unsigned(l) * C::WAVES + wave;
-            lds_load((u % C::UNITS < kHalf ? pb : qb) + size_t(stage) * (C::F * 64) + off[l], buf + u * 1024);
+            lds_load((u % C::UNITS < kHalf ? pb + stage * stage_p : qb + stage * stage_q) + off[l], buf + u * 1024);
         }
         __builtin_amdgcn_sched_barrier(0);
     };
@@ -334,28 +334,28 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.0f;
     const unsigned frag = (lane & 31) * 64, turn = lane >> 2 & 3, unit = (lane >> 5) * 2;
-    auto multiply = [&](const char* stage) {
+    h8 fp[C::TM][2], fq[C::TN][2];
+    auto read = [&](const char* stage) {
+        const char* buf = stage + group * C::SLAB;
 #pragma unroll
-        for (int f = 0; f < C::F / C::KG; ++f) {
-            const char* buf = stage + (f * C::KG + group) * C::SLAB;
-            h8 fp[C::TM][2], fq[C::TN][2];
+        for (int h = 0; h < 2; ++h) {
+            const unsigned at = frag + (((unit + h) ^ turn) * 16);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const unsigned at = frag + (((unit + h) ^ turn) * 16);
+            for (int a = 0; a < C::TM; ++a) fp[a][h] = *reinterpret_cast<const h8*>(buf + (wm + a * 32) * 64 + at);
 #pragma unroll
-                for (int a = 0; a < C::TM; ++a) fp[a][h] = *reinterpret_cast<const h8*>(buf + (wm + a * 32) * 64 + at);
-#pragma unroll
-                for (int b = 0; b < C::TN; ++b) fq[b][h] = *reinterpret_cast<const h8*>(buf + (C::BT + wn + b * 32) * 64 + at);
-            }
-#pragma unroll
-            for (int a = 0; a < C::TM; ++a)
-#pragma unroll
-                for (int b = 0; b < C::TN; ++b) {
-                    acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[a][0], fq[b][0], acc[a][b], 0, 0, 0);
-                    acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[a][0], fq[b][1], acc[a][b], 0, 0, 0);
-                    acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[a][1], fq[b][0], acc[a][b], 0, 0, 0);
-                }
+            for (int b = 0; b < C::TN; ++b) fq[b][h] = *reinterpret_cast<const h8*>(buf + (C::BT + wn + b * 32) * 64 + at);
         }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto multiply = [&]() {
+#pragma unroll
+        for (int a = 0; a < C::TM; ++a)
+#pragma unroll
+            for (int b = 0; b < C::TN; ++b) {
+                acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[a][0], fq[b][0], acc[a][b], 0, 0, 0);
+                acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[a][0], fq[b][1], acc[a][b], 0, 0, 0);
+                acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[a][1], fq[b][0], acc[a][b], 0, 0, 0);
+            }
     };
     // Waits until at most `in_flight` stages of this wave's loads are on their way (they land in order), then
     // for the other waves to have got there: the stage that is multiplied next is in LDS, and every wave is
@@ -374,33 +374,59 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
     typedef std::integral_constant<int, 1> One;
     typedef std::integral_constant<int, 0> None;
     const unsigned stages = k / (16 * C::F);         // k is a multiple of 64, F of 1, 2 or 4
+    // What the epilogue adds to the sums.  A wave of few tiles asks for it now: at the end it would wait for it.
+    auto mine = [&](int tile) { return C::KG == 1 || unsigned(tile) % C::KG == group; };
+    const char* addend = KIND == POLY ? buf_a(j, work) : buf_y(j, work, from);
+    auto addend_at = [&](int a, int b, int quad) {
+        return pair_at(rows_q, j0 + wn + b * 32 + (lane & 31), i0 + wm + a * 32 + quad * 8) + (lane >> 5) * 8;
+    };
+    constexpr bool kEarly = KIND != GRAM && C::TM * C::TN <= 4;
+    h4 old_hi[kEarly ? C::TM : 1][kEarly ? C::TN : 1][4], old_lo[kEarly ? C::TM : 1][kEarly ? C::TN : 1][4];
+    if (kEarly) {
+#pragma unroll
+        for (int a = 0; a < C::TM; ++a)
+#pragma unroll
+            for (int b = 0; b < C::TN; ++b) {
+                if (!mine(a * C::TN + b) || i0 + wm + a * 32 >= rows_p || j0 + wn + b * 32 >= rows_q) continue;
+#pragma unroll
+                for (int quad = 0; quad < 4; ++quad) {
+                    old_hi[kEarly ? a : 0][kEarly ? b : 0][quad] = *reinterpret_cast<const h4*>(addend + addend_at(a, b, quad));
+                    old_lo[kEarly ? a : 0][kEarly ? b : 0][quad] = *reinterpret_cast<const h4*>(addend + addend_at(a, b, quad) + 16);
+                }
+            }
+    }
+    load(s_ring0, 0);
+    if (stages > 1) load(s_ring1, 1);
+    if (C::RING == 4 && stages > 2) load(s_ring2, 2);
+    unsigned s = 0;
     // one stage: how many later ones have been asked for decides the wait
-    auto turn_of = [&](const char* now, char* next, unsigned s) {
+    auto turn_of = [&](const char* now, char* ahead, unsigned s) {
         const unsigned later = stages - 1 - s;
         if (later >= kAhead - 1) arrive(Full{});
         else if (later == 1) arrive(One{});
         else arrive(None{});
-        if (later >= kAhead) load(next, s + kAhead);
-        multiply(now);
+        read(now);
+        if (later >= kAhead) load(ahead, s + kAhead);
+        multiply();
     };
-    load(s_ring0, 0);
-    if (stages > 1) load(s_ring1, 1);
-    if (C::RING == 4 && stages > 2) load(s_ring2, 2);
     if (C::RING == 4) {
-        unsigned s = 0;
-        for (; s + 7 <= stages; s += 4) {            // s + 6 is the last stage that this turn asks for
+        for (; s + 7 <= stages; s += 4) {
             arrive(Full{});
+            read(s_ring0);
             load(s_ring3, s + 3);
-            multiply(s_ring0);
+            multiply();
             arrive(Full{});
+            read(s_ring1);
             load(s_ring0, s + 4);
-            multiply(s_ring1);
+            multiply();
             arrive(Full{});
+            read(s_ring2);
             load(s_ring1, s + 5);
-            multiply(s_ring2);
+            multiply();
             arrive(Full{});
+            read(s_ring3);
             load(s_ring2, s + 6);
-            multiply(s_ring3);
+            multiply();
         }
         for (; s < stages; s += 4) {
             turn_of(s_ring0, s_ring3, s);
@@ -409,17 +435,19 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
             if (s + 3 < stages) turn_of(s_ring3, s_ring2, s + 3);
         }
     } else {
-        unsigned s = 0;
         for (; s + 5 <= stages; s += 3) {
             arrive(Full{});
+            read(s_ring0);
             load(s_ring2, s + 2);
-            multiply(s_ring0);
+            multiply();
             arrive(Full{});
+            read(s_ring1);
             load(s_ring0, s + 3);
-            multiply(s_ring1);
+            multiply();
             arrive(Full{});
+            read(s_ring2);
             load(s_ring1, s + 4);
-            multiply(s_ring2);
+            multiply();
         }
         for (; s < stages; s += 3) {
             turn_of(s_ring0, s_ring2, s);
@@ -435,7 +463,6 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
         return (ring == 0 ? s_ring0 : ring == 1 ? s_ring1 : ring == 2 ? s_ring2 : s_ring3) + (i % kPieces) * 4096;
     };
     // The groups of a position add their sums: tile t of the wave's goes to group t % KG, in group order.
-    auto mine = [&](int tile) { return C::KG == 1 || unsigned(tile) % C::KG == group; };
     if (C::KG > 1) {
         constexpr int kTiles = C::TM * C::TN;
 #pragma unroll
@@ -475,10 +502,8 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
 
     // accumulator register e of a lane: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32 of its 32 x 32 tile
     const bool mirror = !SYM || ti != tj;            // a tile on the diagonal is its own mirror image
-    const unsigned ld_direct = SYM ? rows_p : rows_q, ld_turned = rows_p;
     char* direct = KIND == GRAM ? buf_a(j, work) : KIND == POLY ? buf_b(j, work) : buf_x(j, work, from ^ 1);
     char* turned = KIND == GRAM ? buf_a(j, work) : KIND == POLY ? buf_b(j, work) : buf_y(j, work, from ^ 1);
-    const char* addend = KIND == POLY ? buf_a(j, work) : buf_y(j, work, from);
     uint32_t* s_turn = reinterpret_cast<uint32_t*>(piece(wave));       // a 32 x 32 tile per wave is turned in LDS
     const unsigned half = lane >> 5, col = lane & 31;
 #pragma unroll
@@ -489,7 +514,7 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
             if (!mine(a * C::TN + b) || gi >= rows_p || gj >= rows_q) continue;     // wave-uniform; rows are multiples of 64
 #pragma unroll
             for (int quad = 0; quad < 4; ++quad) {
-                const size_t at = (size_t(gj + col) * ld_turned + gi) * 4 + quad * 32 + half * 8;
+                const size_t at = pair_at(rows_q, gj + col, gi + quad * 8) + half * 8;
                 float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = acc[a][b][quad * 4 + e];
@@ -497,7 +522,8 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] *= kScaleA / (kScaleX * kScaleX);
                 } else {
-                    const h4 oh = *reinterpret_cast<const h4*>(addend + at), ol = *reinterpret_cast<const h4*>(addend + at + 16);
+                    const h4 oh = kEarly ? old_hi[kEarly ? a : 0][kEarly ? b : 0][quad] : *reinterpret_cast<const h4*>(addend + addend_at(a, b, quad));
+                    const h4 ol = kEarly ? old_lo[kEarly ? a : 0][kEarly ? b : 0][quad] : *reinterpret_cast<const h4*>(addend + addend_at(a, b, quad) + 16);
                     const float f = KIND == POLY ? cc / kScaleA : KIND == STEP ? 1.0f / kScaleA : 1.0f / (kScaleA * kScaleX);
                     const float old = KIND == POLY ? cb : KIND == STEP ? ca : ca / kScaleX;
 #pragma unroll
@@ -535,7 +561,7 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const unsigned row = (lane >> 2) + 16 * h, c8 = lane & 3;
+                const unsigned row = lane >> 1, c8 = 2 * h + (lane & 1);
                 const u4 w0 = *reinterpret_cast<const u4*>(s_turn + row * 32 + (((2 * c8) ^ row) & 7) * 4);
                 const u4 w1 = *reinterpret_cast<const u4*>(s_turn + row * 32 + (((2 * c8 + 1) ^ row) & 7) * 4);
                 u4 hi, lo;
@@ -547,7 +573,7 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
                 lo[1] = (w0[2] >> 16) | (w0[3] & 0xffff0000u);
                 lo[2] = (w1[0] >> 16) | (w1[1] & 0xffff0000u);
                 lo[3] = (w1[2] >> 16) | (w1[3] & 0xffff0000u);
-                u4* dst = reinterpret_cast<u4*>(direct + (size_t(gi + row) * ld_direct + gj + c8 * 8) * 4);
+                u4* dst = reinterpret_cast<u4*>(direct + pair_at(rows_p, gi + row, gj + c8 * 8));
                 dst[0] = hi;
                 dst[1] = lo;
             }
@@ -562,43 +588,50 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
 // through the contracted rows in that order: X enters B X as it stands, and so do the symmetric A and B, which
 // are their own transposes.  Only X X^T contracts over the lanes; there the tile is turned by a product with
 // the identity, exact in fp32.  So X stays in registers through all steps, in fp32 (times 2^13), and LDS
-// carries nothing but the waves' shares of X X^T and, with four tiles, of A A.  The two low halves' product
-// is included: it costs nothing here.
+// carries nothing but the waves' shares of X X^T and, with four tiles, of A A.
+// With up to 32 rows a pair's 22 bits would show: the sums are too short for fp32's own roundings to hide
+// them (256 x 10: 1.0e-6 from 64 bits against 0.67e-6 by fp32 products).  There numbers are kept in three
+// parts, all 24 bits, and a product is six MFMAs; from 33 rows on pairs and three MFMAs come out alike.
 // A matrix of one stripe (a block's columns) goes through all its steps in one launch; with more stripes, a
 // launch per step: every block adds the stripes' shares for itself, in order.
 enum NarrowMode { WHOLE, FIRST, NEXT };
 constexpr unsigned kTileFloats = 1024;
 
-struct Pairs {                                        // an operand of 32 contracted rows: two MFMA steps
-    h8 hi[2], lo[2];
+// An operand of 32 contracted rows (two MFMA steps) as N f16 parts: two hold 22 bits of a float, three all 24.
+template <int N>
+struct Parts {
+    h8 part[N][2];
 };
-__device__ __forceinline__ Pairs pairs_of(const float (&v)[16]) {
+template <int N>
+__device__ __forceinline__ Parts<N> parts_of(const float (&v)[16]) {
     typedef _Float16 h2 __attribute__((ext_vector_type(2)));
     typedef float v2f __attribute__((ext_vector_type(2)));
-    Pairs r;
+    Parts<N> r;
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-            const v2f x = {v[8 * s + e], v[8 * s + e + 1]};
-            const h2 h = __builtin_convertvector(x, h2);
-            const v2f d = {x[0] - float(h[0]), x[1] - float(h[1])};
-            const h2 l = __builtin_convertvector(d, h2);
-            r.hi[s][e] = h[0];
-            r.hi[s][e + 1] = h[1];
-            r.lo[s][e] = l[0];
-            r.lo[s][e + 1] = l[1];
+            v2f x = {v[8 * s + e], v[8 * s + e + 1]};
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const h2 h = __builtin_convertvector(x, h2);
+                r.part[n][s][e] = h[0];
+                r.part[n][s][e + 1] = h[1];
+                x[0] -= float(h[0]);
+                x[1] -= float(h[1]);
+            }
         }
     return r;
 }
-__device__ __forceinline__ void multiply_pairs(v16f& acc, const Pairs& p, const Pairs& q) {
+// the products of parts whose places add up to less than N: what is left out is below 2^(-11 N)
+template <int N>
+__device__ __forceinline__ void multiply_parts(v16f& acc, const Parts<N>& p, const Parts<N>& q) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p.lo[s], q.lo[s], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p.hi[s], q.lo[s], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p.lo[s], q.hi[s], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p.hi[s], q.hi[s], acc, 0, 0, 0);
-    }
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int sum = N - 1; sum >= 0; --sum)
+#pragma unroll
+            for (int i = 0; i <= sum; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p.part[i][s], q.part[sum - i][s], acc, 0, 0, 0);
 }
 __device__ __forceinline__ v16f zero16() {
     v16f z;
@@ -627,6 +660,7 @@ __device__ __forceinline__ void add_tile(const float* from, unsigned lane, float
 template <int ROWS_, int WAVES_>
 struct NarrowCfg {
     static constexpr int ROWS = ROWS_, WAVES = WAVES_, STRIPE = 32 * WAVES_, TILES = ROWS * ROWS, THREADS = 64 * WAVES_;
+    static constexpr int N = ROWS == 1 ? 3 : 2;       // parts of a number
     // ROWS == 1: the waves' shares twice (a wave may be a step ahead of another that still reads).
     // ROWS == 2: the shares - and in their place, later in a step, the parts of A A - and their sum.
     static constexpr int SHARES = ROWS == 1 ? 2 * WAVES : WAVES * TILES;
@@ -655,7 +689,7 @@ __device__ inline unsigned left_of(const Job& j, unsigned stripe, unsigned wide)
 // NEXT: one step; `last` writes the result.
 template <NarrowMode MODE, class C>
 __global__ __launch_bounds__(C::THREADS) void narrow_product(Table t, int steps, int parity, int last, float ca, float cb, float cc) {
-    constexpr int ROWS = C::ROWS, TILES = C::TILES, WAVES = C::WAVES;
+    constexpr int ROWS = C::ROWS, TILES = C::TILES, WAVES = C::WAVES, N = C::N;
     __shared__ __attribute__((aligned(16))) float s_share[C::SHARES * kTileFloats];
     __shared__ __attribute__((aligned(16))) float s_sum[TILES * kTileFloats];
     __shared__ double s_part[WAVES];
@@ -796,33 +830,32 @@ __global__ __launch_bounds__(C::THREADS) void narrow_product(Table t, int steps,
 #pragma unroll
         for (int e = 0; e < 8; ++e) eye[s][e] = row_of(0, 8 * s + e) == (lane & 31) ? _Float16(1) : _Float16(0);
 
-    Pairs xp[ROWS];
-    auto pair_x = [&]() {
+    Parts<N> xp[ROWS];
+    auto part_x = [&]() {
 #pragma unroll
-        for (int a = 0; a < ROWS; ++a) xp[a] = pairs_of(x[a]);
+        for (int a = 0; a < ROWS; ++a) xp[a] = parts_of<N>(x[a]);
     };
     // this wave's share of X X^T to LDS, from the turned tiles
     auto put_shares = [&](float* shares) {
-        Pairs xt[ROWS];
+        Parts<N> xt[ROWS];
 #pragma unroll
         for (int a = 0; a < ROWS; ++a) {
             v16f acc = zero16();
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(xp[a].hi[s], eye[s], acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(xp[a].lo[s], eye[s], acc, 0, 0, 0);
-            }
+            for (int n = N - 1; n >= 0; --n)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(xp[a].part[n][s], eye[s], acc, 0, 0, 0);
             float v[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) v[e] = acc[e];
-            xt[a] = pairs_of(v);
+            xt[a] = parts_of<N>(v);
         }
 #pragma unroll
         for (int a = 0; a < ROWS; ++a)
 #pragma unroll
             for (int b = 0; b < ROWS; ++b) {
                 v16f acc = zero16();
-                multiply_pairs(acc, xt[a], xt[b]);
+                multiply_parts<N>(acc, xt[a], xt[b]);
                 float v[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) v[e] = acc[e] * (1.0f / (kScaleX * kScaleX));
@@ -856,14 +889,14 @@ __global__ __launch_bounds__(C::THREADS) void narrow_product(Table t, int steps,
             float v[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) v[e] = a[e] * kScaleA;
-            const Pairs ap = pairs_of(v);
+            const Parts<N> ap = parts_of<N>(v);
             v16f acc = zero16();
-            multiply_pairs(acc, ap, ap);
+            multiply_parts<N>(acc, ap, ap);
 #pragma unroll
             for (int e = 0; e < 16; ++e) v[e] = (cb * a[e] + acc[e] * (cc / (kScaleA * kScaleA))) * kScaleA;
-            const Pairs bp = pairs_of(v);
+            const Parts<N> bp = parts_of<N>(v);
             acc = zero16();
-            multiply_pairs(acc, bp, xp[0]);
+            multiply_parts<N>(acc, bp, xp[0]);
 #pragma unroll
             for (int e = 0; e < 16; ++e) x[0][e] = ca * x[0][e] + acc[e] * (1.0f / kScaleA);
             return;
@@ -884,13 +917,13 @@ __global__ __launch_bounds__(C::THREADS) void narrow_product(Table t, int steps,
                 q[e] *= kScaleA;
             }
             v16f acc = zero16();
-            multiply_pairs(acc, pairs_of(p), pairs_of(q));
+            multiply_parts<N>(acc, parts_of<N>(p), parts_of<N>(q));
 #pragma unroll
             for (int e = 0; e < 16; ++e) v[e] = (cb * v[e] + acc[e] * (cc / (kScaleA * kScaleA))) * kScaleA;
             put_tile(s_share + wave * kTileFloats, lane, v);
         }
         __syncthreads();
-        Pairs bp[TILES];
+        Parts<N> bp[TILES];
 #pragma unroll
         for (int i = 0; i < TILES; ++i) {
             float v[16];
@@ -898,14 +931,14 @@ __global__ __launch_bounds__(C::THREADS) void narrow_product(Table t, int steps,
             for (int e = 0; e < 16; ++e) v[e] = 0.0f;
             add_tile(s_share + i * kTileFloats, lane, v);
             add_tile(s_share + (4 + i) * kTileFloats, lane, v);
-            bp[i] = pairs_of(v);
+            bp[i] = parts_of<N>(v);
         }
         __syncthreads();                              // the next shares overwrite the parts
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             v16f acc = zero16();
 #pragma unroll
-            for (int k = 0; k < ROWS; ++k) multiply_pairs(acc, bp[k * ROWS + r], xp[k]);
+            for (int k = 0; k < ROWS; ++k) multiply_parts<N>(acc, bp[k * ROWS + r], xp[k]);
 #pragma unroll
             for (int e = 0; e < 16; ++e) x[r][e] = ca * x[r][e] + acc[e] * (1.0f / kScaleA);
         }
@@ -914,7 +947,7 @@ __global__ __launch_bounds__(C::THREADS) void narrow_product(Table t, int steps,
     if (MODE == WHOLE) {
 #pragma unroll 1
         for (int s = 0; s < steps; ++s) {
-            pair_x();
+            part_x();
             float* shares = s_share + (ROWS == 1 ? (s & 1) * WAVES * int(kTileFloats) : 0);
             put_shares(shares);
             __syncthreads();
@@ -935,7 +968,7 @@ __global__ __launch_bounds__(C::THREADS) void narrow_product(Table t, int steps,
             const float* from = narrow_shares(j, work, parity);
             for (unsigned i = threadIdx.x; i < TILES * kTileFloats / 4; i += C::THREADS)
                 *reinterpret_cast<v4f*>(s_sum + i * 4) = joint_sum(from, stripes, TILES * kTileFloats, i);
-            pair_x();
+            part_x();
             __syncthreads();
             if (ROWS == 1) {
 #pragma unroll
@@ -945,7 +978,7 @@ __global__ __launch_bounds__(C::THREADS) void narrow_product(Table t, int steps,
             step(a);
         }
         if (!last) {
-            pair_x();
+            part_x();
             put_shares(s_share);
             if (live)
 #pragma unroll
@@ -1023,6 +1056,7 @@ void shape_job(Job* j, int64_t rows, int64_t cols, unsigned count) {
     if (j->m <= 64 && narrow > j->work_stride) j->work_stride = narrow;
 }
 
+typedef TileCfg<32, 32, 32, 4, 4, 4> Tile32;
 typedef TileCfg<64, 32, 32, 4, 4, 4> Tile64;
 typedef TileCfg<128, 64, 64, 2, 2, 4> Tile128;
 typedef TileCfg<192, 96, 96, 2, 2, 3> Tile192;
@@ -1047,21 +1081,30 @@ unsigned sym_tiles(const Job& j, unsigned bt) {
 }
 unsigned full_tiles(const Job& j, unsigned bt) { return ((unsigned(j.mp) + bt - 1) / bt) * ((unsigned(j.np) + bt - 1) / bt); }
 
-// The tile of a launch: the one whose rounds of one block per CU cost least.
+// The tile of a launch: the one whose rounds over the chip cost least.  The cost of a round is the time a
+// block takes per k, measured (us per 1024 k, launch taken off, one block on every CU): a small tile waits
+// for its loads, a large one for the matrix cores - 4 times the work in 2.3 times the time from 64 to 128.
+//   4096 x 4096, X X^T: 253 tiles of 192 in 205 us, 136 of 256 in 265, 528 of 128 in 258;  B X: 256 tiles of
+//   256 in 350 us, 484 of 192 in 417;  2048 x 2048: 136 of 128 in 48 us, 528 of 64 in 57, 66 of 192 in 81;
+//   1024 x 1024: 136 of 64 in 12 us, 36 of 128 in 23;  333 x 1000: 78 of 32 in 8.6 us, 21 of 64 in 11.4.
 template <class F>
 int pick_tile(const Table& t, F tiles) {
     const size_t cus = size_t(compute_units() > 0 ? compute_units() : 256);
-    const int sizes[4] = {256, 192, 128, 64};
-    const double cost[4] = {16.0, 9.6, 5.0, 1.9};
-    int best = 256;
+    struct Choice {
+        int tile, resident;                           // blocks per CU (by LDS)
+        double cost;
+    };
+    const Choice choices[5] = {{256, 1, 64.0}, {192, 1, 38.0}, {128, 1, 18.0}, {64, 1, 8.0}, {32, 2, 5.5}};
+    int best = 0;
     double least = 1e300;
-    for (int i = 0; i < 4; ++i) {
+    for (const Choice& c : choices) {
         size_t blocks = 0;
-        for (int j = 0; j < t.jobs; ++j) blocks += size_t(t.job[j].count) * tiles(t.job[j], unsigned(sizes[i]));
-        const double c = double((blocks + cus - 1) / cus) * cost[i];
-        if (c < least) {
-            least = c;
-            best = sizes[i];
+        for (int j = 0; j < t.jobs; ++j) blocks += size_t(t.job[j].count) * tiles(t.job[j], unsigned(c.tile));
+        const size_t at_once = cus * size_t(c.resident);
+        const double cost = double((blocks + at_once - 1) / at_once) * c.cost;
+        if (cost < least) {
+            least = cost;
+            best = c.tile;
         }
     }
     return best;
@@ -1077,7 +1120,8 @@ void launch_product(int tile, Table* t, int from, const float* c, hipStream_t s)
     if (tile == 256) launch_product<Tile256, KIND>(t, from, c, s);
     else if (tile == 192) launch_product<Tile192, KIND>(t, from, c, s);
     else if (tile == 128) launch_product<Tile128, KIND>(t, from, c, s);
-    else launch_product<Tile64, KIND>(t, from, c, s);
+    else if (tile == 64) launch_product<Tile64, KIND>(t, from, c, s);
+    else launch_product<Tile32, KIND>(t, from, c, s);
 }
 
 int iterate(const char* who, Table* t, int steps, const float* c, hipStream_t s) {
