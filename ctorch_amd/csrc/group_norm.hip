@@ -17,8 +17,9 @@
 // takes the mean of the values it holds, then their squared deviations, and parts are joined by
 //   M2 = M2a + M2b + (mean_a - mean_b)^2 na nb / (na + nb),
 // so a group whose mean is large against its deviation keeps its digits.
+#include <type_traits>
+
 #include "common.h"
-#include "devmath.h"
 
 namespace ctamd {
 namespace {
@@ -30,17 +31,17 @@ template <int V>
 struct Vec {
     float v[V];
 };
-template <int V>
+// STREAM: with the hint that the line is not wanted again
+template <int V, bool STREAM = false>
 __device__ __forceinline__ Vec<V> load_vec(const float* p) {
     typedef float vt __attribute__((ext_vector_type(V)));
-    const vt t = *reinterpret_cast<const vt*>(p);
+    const vt* q = reinterpret_cast<const vt*>(p);
+    const vt t = STREAM ? __builtin_nontemporal_load(q) : *q;
     Vec<V> r;
 #pragma unroll
     for (int i = 0; i < V; ++i) r.v[i] = t[i];
     return r;
 }
-template <>
-__device__ __forceinline__ Vec<1> load_vec<1>(const float* p) { return {{*p}}; }
 template <int V>
 __device__ __forceinline__ void store_vec(float* p, const Vec<V>& a) {
     typedef float vt __attribute__((ext_vector_type(V)));
@@ -60,23 +61,33 @@ __device__ __forceinline__ Vec<V> affine_vec(const float* p, size_t at, float wi
     return r;
 }
 
-// 1 / (1 + e^-z) in single precision for any z (e^-z past the largest float gives 0, NaN stays NaN)
+// 1 / (1 + e^-z) in single precision, z >= -80 (or NaN): the exponential as in devmath.h, the hardware's
+// reciprocal (1 ulp); within 3 ulp.  The two transcendental instructions take half of its time.
 __device__ __forceinline__ float logistic(float z) {
-    const float s = 1.0f + cta_exp_hw(-z);
-    return s > 1e38f ? 0.0f : cta_rcp_refined(s);
+    const float d = -fminf(z, 100.0f), p = d * 0x1.715476p+0f;
+    const float e = __builtin_amdgcn_exp2f(p);
+    float t = __fmaf_rn(p, -0x1.62e4p-1f, d);
+    t = __fmaf_rn(p, -0x1.7f7d1cp-20f, t);
+    return __builtin_amdgcn_rcpf(1.0f + __fmaf_rn(e, t, e));
 }
+// SiLU and its slope are below 2e-33 left of -80: z goes no further, which keeps e^-z and z (1 - s) finite
+__device__ __forceinline__ float silu_range(float z) { return z < -80.0f ? -80.0f : z; }
 template <int ACT>
 __device__ __forceinline__ float activate(float z) {
     if (ACT == CTAMD_ACT_RELU) return z > 0.0f ? z : 0.0f;
-    if (ACT == CTAMD_ACT_SILU) return z * logistic(z);
+    if (ACT == CTAMD_ACT_SILU) {
+        z = silu_range(z);
+        return z * logistic(z);
+    }
     return z;
 }
 // g act'(z); z is only formed where an activation needs it
 template <int ACT>
 __device__ __forceinline__ float activate_grad(float xhat, float w, float b, float g) {
     if (ACT == CTAMD_ACT_NONE) return g;
-    const float z = xhat * w + b;
+    float z = xhat * w + b;
     if (ACT == CTAMD_ACT_RELU) return z > 0.0f ? g : g * 0.0f;
+    z = silu_range(z);
     const float s = logistic(z);
     return g * (s * (1.0f + z * (1.0f - s)));
 }
@@ -250,6 +261,7 @@ struct Tile {
     unsigned block_groups;        // groups per block (1 when pieces > 1)
     unsigned pieces;              // blocks that share one group
     unsigned col_blocks;          // blocks along the channels
+    unsigned join_lanes;          // lanes that join one group's sums (a power of two, at most 64)
     unsigned chunks;              // blocks along the positions (1: resident)
     size_t chunk_rows;
 };
@@ -308,8 +320,9 @@ __device__ __forceinline__ Moments join(const Moments& a, const Moments& b) {
     return r;
 }
 
-// Joins the moments of a block's threads per group; wave w takes the groups w, w + waves, ...  The mean
-// first (a sum of n mean), then the deviations from it.  every(group, moments) is called by lane 0.
+// Joins the moments of a block's threads per group, all groups at once: a power of two of lanes to each.
+// The mean first (a sum of n mean), then the deviations from it.  every(group, moments) is called by one lane
+// per group.
 template <int V, int T, class F>
 __device__ __forceinline__ void join_groups(const Tile& t, const Place& p, float* s_mean, float* s_m2, float* s_n, const Moments& mine, F every) {
     s_mean[threadIdx.x] = mine.mean;
@@ -318,25 +331,28 @@ __device__ __forceinline__ void join_groups(const Tile& t, const Place& p, float
     __syncthreads();
     const unsigned per = t.pieces > 1 ? p.cols : t.width / V;              // vectors of a group in this block
     const unsigned here = t.pieces > 1 ? 1 : p.cols / per;
-    const unsigned wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const unsigned lanes = t.join_lanes, lane = threadIdx.x & (lanes - 1);
     const unsigned entries = per * t.row_lanes;
-    for (unsigned g = wave; g < here; g += T / 64) {
+    for (unsigned g0 = 0; g0 < here; g0 += T / lanes) {                     // uniform: the shuffles want whole waves
+        const unsigned g = g0 + threadIdx.x / lanes;
+        const bool in = g < here;
         float n = 0.0f, s = 0.0f;
-        for (unsigned e = lane; e < entries; e += 64) {
-            const unsigned at = (e / per) * t.cols + g * per + e % per;
+        for (unsigned e = lane; e < entries; e += lanes) {
+            const unsigned at = in ? (e / per) * t.cols + g * per + e % per : 0;
             n += s_n[at];
             s += s_n[at] * s_mean[at];
         }
-        n = lanes_sum(n, 64);
-        const float mean = n > 0.0f ? lanes_sum(s, 64) / n : 0.0f;
+        n = lanes_sum(n, int(lanes));
+        s = lanes_sum(s, int(lanes));
+        const float mean = n > 0.0f ? s / n : 0.0f;
         float m2 = 0.0f;
-        for (unsigned e = lane; e < entries; e += 64) {
-            const unsigned at = (e / per) * t.cols + g * per + e % per;
+        for (unsigned e = lane; e < entries; e += lanes) {
+            const unsigned at = in ? (e / per) * t.cols + g * per + e % per : 0;
             const float d = s_mean[at] - mean;
             m2 += s_n[at] > 0.0f ? s_m2[at] + s_n[at] * (d * d) : 0.0f;
         }
-        m2 = lanes_sum(m2, 64);
-        if (lane == 0) every(g, Moments{n, mean, m2});
+        m2 = lanes_sum(m2, int(lanes));
+        if (in && lane == 0) every(g, Moments{n, mean, m2});
     }
 }
 
@@ -356,7 +372,7 @@ __device__ __forceinline__ Moments moments_of(const Vec<V> (&v)[K], int count) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const float d = v[k].v[i] - m.mean;
-            m.m2 += k < count ? d * d : 0.0f;
+            m.m2 = k < count ? __fmaf_rn(d, d, m.m2) : m.m2;
         }
     return m;
 }
@@ -402,7 +418,7 @@ __global__ __launch_bounds__(T) void resident_forward(Tile t, const float* x, co
 
 // parts[((n * groups + group) * pieces + piece) * chunks + chunk] = (mean, M2) of that part of the group
 constexpr int kStatRows = 8;
-template <int V>
+template <int V, bool STREAM>
 __global__ __launch_bounds__(kT) void split_stats(Tile t, const float* __restrict__ x, float* __restrict__ parts) {
     __shared__ float s_mean[kT], s_m2[kT], s_n[kT];
     const Place p = place<V, kT>(t, blockIdx.x);
@@ -411,14 +427,15 @@ __global__ __launch_bounds__(kT) void split_stats(Tile t, const float* __restric
         const float* src = x + (p.n * t.positions + p.first + p.row) * t.channels + p.col0 + p.col * V;
         const size_t step = size_t(t.row_lanes) * t.channels;
         size_t left = rows_of(p.first + p.row, p.last, t.row_lanes);
-        for (; left > 0; src += kStatRows * step) {
-            const int count = left < kStatRows ? int(left) : kStatRows;
+        auto batch = [&](auto full) {
+            const int count = decltype(full)::value ? kStatRows : int(left);
             Vec<V> v[kStatRows];
 #pragma unroll
-            for (int k = 0; k < kStatRows; ++k) v[k] = k < count ? load_vec<V>(src + k * step) : Vec<V>{};
+            for (int k = 0; k < kStatRows; ++k) v[k] = k < count ? load_vec<V, STREAM>(src + k * step) : Vec<V>{};
             run = join(run, moments_of<V, kStatRows>(v, count));
-            left -= count;
-        }
+        };
+        for (; left >= kStatRows; src += kStatRows * step, left -= kStatRows) batch(std::true_type{});
+        if (left > 0) batch(std::false_type{});
     }
     join_groups<V, kT>(t, p, s_mean, s_m2, s_n, run, [&](unsigned g, const Moments& m) {
         float* o = parts + 2 * (((p.n * t.groups + p.group0 + g) * t.pieces + p.piece) * t.chunks + p.chunk);
@@ -427,12 +444,10 @@ __global__ __launch_bounds__(kT) void split_stats(Tile t, const float* __restric
     });
 }
 
-// One wave per (sample, group): the parts of its chunks and pieces, whose sizes follow from the tile.
+// The statistics of one (sample, group) from its parts, whose sizes follow from the tile, by `lanes`
+// neighbouring lanes: every one of them gets (mean, rstd).
 template <int V>
-__global__ __launch_bounds__(kT) void split_join(Tile t, const float* __restrict__ parts, float eps, float* __restrict__ stats) {
-    const size_t unit = size_t(blockIdx.x) * kWaves + (threadIdx.x >> 6);
-    const unsigned lane = threadIdx.x & 63;
-    if (unit >= t.samples * t.groups) return;
+__device__ __forceinline__ void join_parts(const Tile& t, const float* parts, size_t unit, float eps, unsigned lane, unsigned lanes, float* mean, float* rstd) {
     const unsigned entries = t.pieces * t.chunks;
     const float* src = parts + 2 * unit * entries;
     auto size_of = [&](unsigned e) {
@@ -449,39 +464,73 @@ __global__ __launch_bounds__(kT) void split_join(Tile t, const float* __restrict
     };
     const float whole = float(t.positions * t.width);
     float s = 0.0f;
-    for (unsigned e = lane; e < entries; e += 64) s += size_of(e) * src[2 * e];
-    const float mean = lanes_sum(s, 64) / whole;
+#pragma unroll 4
+    for (unsigned e = lane; e < entries; e += lanes) s += size_of(e) * src[2 * e];
+    const float m = lanes_sum(s, int(lanes)) / whole;
     float m2 = 0.0f;
-    for (unsigned e = lane; e < entries; e += 64) {
-        const float d = src[2 * e] - mean;
+#pragma unroll 4
+    for (unsigned e = lane; e < entries; e += lanes) {
+        const float d = src[2 * e] - m;
         m2 += src[2 * e + 1] + size_of(e) * (d * d);
     }
-    m2 = lanes_sum(m2, 64);
+    *mean = m;
+    *rstd = inv_sqrt(lanes_sum(m2, int(lanes)) / whole, eps);
+}
+// One wave per (sample, group).
+template <int V>
+__global__ __launch_bounds__(kT) void split_join(Tile t, const float* __restrict__ parts, float eps, float* __restrict__ stats) {
+    const size_t unit = size_t(blockIdx.x) * kWaves + (threadIdx.x >> 6);
+    const unsigned lane = threadIdx.x & 63;
+    if (unit >= t.samples * t.groups) return;
+    float mean, rstd;
+    join_parts<V>(t, parts, unit, eps, lane, 64, &mean, &rstd);
     if (lane == 0) {
         stats[2 * unit] = mean;
-        stats[2 * unit + 1] = inv_sqrt(m2 / whole, eps);
+        stats[2 * unit + 1] = rstd;
     }
 }
 
 constexpr int kApplyRows = 4;
-template <int V, int ACT>
+template <int V, int ACT, bool STREAM>
 __global__ __launch_bounds__(kT) void split_apply(Tile t, const float* x, const float* __restrict__ weight, const float* __restrict__ bias,
-                                                  const float* __restrict__ stats, float* y) {
+                                                  float* stats, const float* __restrict__ parts, float eps, float* y) {
+    __shared__ float s_stat[kT][2];
     const Place p = place<V, kT>(t, blockIdx.x);
-    if (!p.live) return;
     const unsigned g = t.pieces > 1 ? 0 : p.col / (t.width / V);
-    const float* st = stats + 2 * (p.n * t.groups + p.group0 + g);
-    const float mean = st[0], rstd = st[1];
+    float mean = 0.0f, rstd = 0.0f;
+    if (parts) {                                      // few enough that every block joins its groups' parts itself
+        const unsigned here = t.pieces > 1 ? 1 : p.cols / (t.width / V);
+        const unsigned lane = threadIdx.x & (t.join_lanes - 1);
+        for (unsigned g0 = 0; g0 < here; g0 += kT / t.join_lanes) {
+            const unsigned gi = g0 + threadIdx.x / t.join_lanes, unit_g = p.group0 + (gi < here ? gi : 0);
+            join_parts<V>(t, parts, p.n * t.groups + unit_g, eps, lane, t.join_lanes, &mean, &rstd);
+            if (gi < here && lane == 0) {
+                s_stat[gi][0] = mean;
+                s_stat[gi][1] = rstd;
+                if (stats && p.chunk == 0 && p.piece == 0) {
+                    stats[2 * (p.n * t.groups + unit_g)] = mean;
+                    stats[2 * (p.n * t.groups + unit_g) + 1] = rstd;
+                }
+            }
+        }
+        __syncthreads();
+        mean = s_stat[g][0];
+        rstd = s_stat[g][1];
+    } else if (p.live) {
+        mean = stats[2 * (p.n * t.groups + p.group0 + g)];
+        rstd = stats[2 * (p.n * t.groups + p.group0 + g) + 1];
+    }
+    if (!p.live) return;
     const Vec<V> w = affine_vec<V>(weight, p.col0 + p.col * V, 1.0f), b = affine_vec<V>(bias, p.col0 + p.col * V, 0.0f);
     const float* src = x + (p.n * t.positions + p.first + p.row) * t.channels + p.col0 + p.col * V;
     float* dst = y + (src - x);
     const size_t step = size_t(t.row_lanes) * t.channels;
     size_t left = rows_of(p.first + p.row, p.last, t.row_lanes);
-    for (; left > 0; src += kApplyRows * step, dst += kApplyRows * step) {
-        const int count = left < kApplyRows ? int(left) : kApplyRows;
+    auto batch = [&](auto full) {
+        const int count = decltype(full)::value ? kApplyRows : int(left);
         Vec<V> v[kApplyRows];
 #pragma unroll
-        for (int k = 0; k < kApplyRows; ++k) v[k] = k < count ? load_vec<V>(src + k * step) : Vec<V>{};
+        for (int k = 0; k < kApplyRows; ++k) v[k] = k < count ? load_vec<V, STREAM>(src + k * step) : Vec<V>{};
 #pragma unroll
         for (int k = 0; k < kApplyRows; ++k)
             if (k < count) {
@@ -490,8 +539,9 @@ __global__ __launch_bounds__(kT) void split_apply(Tile t, const float* x, const 
                 for (int i = 0; i < V; ++i) o.v[i] = activate<ACT>((v[k].v[i] - mean) * rstd * w.v[i] + b.v[i]);
                 store_vec<V>(dst + k * step, o);
             }
-        left -= count;
-    }
+    };
+    for (; left >= kApplyRows; src += kApplyRows * step, dst += kApplyRows * step, left -= kApplyRows) batch(std::true_type{});
+    if (left > 0) batch(std::false_type{});
 }
 
 // Adds the row lanes of a block per channel: the threads of row lane 0 receive the sums of a and b.
@@ -605,11 +655,14 @@ __global__ __launch_bounds__(T) void resident_backward(Tile t, const float* x, c
 }
 
 // parts[(n * chunks + chunk)][2][C]: sums over the chunk's positions of dz xhat and dz, per channel
-constexpr int kGradRows = 4;
-template <int V, int ACT>
+// rows of x and g that a thread loads at once: more where they come from HBM (512 MiB: 226 us with 8, 234 with 4;
+// 128 MiB from the cache: 73 and 69)
+constexpr int grad_rows(bool stream) { return stream ? 8 : 4; }
+template <int V, int ACT, bool STREAM>
 __global__ __launch_bounds__(kT) void split_grad_sums(Tile t, const float* __restrict__ x, const float* __restrict__ weight,
                                                       const float* __restrict__ bias, const float* __restrict__ stats,
                                                       const float* __restrict__ g_out, float* __restrict__ parts, size_t n0) {
+    constexpr int kGradRows = grad_rows(STREAM);
     __shared__ float s_red[2 * V][kT];
     const Place p = place<V, kT>(t, blockIdx.x);
     Vec<V> sw{}, sb{};
@@ -621,13 +674,13 @@ __global__ __launch_bounds__(kT) void split_grad_sums(Tile t, const float* __res
         size_t at = ((n0 + p.n) * t.positions + p.first + p.row) * t.channels + p.col0 + p.col * V;
         const size_t step = size_t(t.row_lanes) * t.channels;
         size_t left = rows_of(p.first + p.row, p.last, t.row_lanes);
-        for (; left > 0; at += kGradRows * step) {
-            const int count = left < kGradRows ? int(left) : kGradRows;
+        auto batch = [&](auto full) {
+            const int count = decltype(full)::value ? kGradRows : int(left);
             Vec<V> h[kGradRows], d[kGradRows];
 #pragma unroll
             for (int k = 0; k < kGradRows; ++k) {
-                h[k] = k < count ? load_vec<V>(x + at + k * step) : Vec<V>{};
-                d[k] = k < count ? load_vec<V>(g_out + at + k * step) : Vec<V>{};
+                h[k] = k < count ? load_vec<V, STREAM>(x + at + k * step) : Vec<V>{};
+                d[k] = k < count ? load_vec<V, STREAM>(g_out + at + k * step) : Vec<V>{};
             }
             Vec<V> tw{}, tb{};                     // a turn's terms first, then the running sum: shorter chains of roundings
 #pragma unroll
@@ -644,8 +697,9 @@ __global__ __launch_bounds__(kT) void split_grad_sums(Tile t, const float* __res
                 sw.v[i] += tw.v[i];
                 sb.v[i] += tb.v[i];
             }
-            left -= count;
-        }
+        };
+        for (; left >= kGradRows; at += kGradRows * step, left -= kGradRows) batch(std::true_type{});
+        if (left > 0) batch(std::false_type{});
     }
     add_row_lanes<V, kT>(t, p, s_red, sw, sb);
     if (p.live && p.row == 0) {
@@ -658,60 +712,75 @@ __global__ __launch_bounds__(kT) void split_grad_sums(Tile t, const float* __res
     }
 }
 
-// One wave per (sample, group): the chunks' sums per channel, kept in sums[n][2][C] for dweight and
-// dbias, and the group's s1, s2.
-__global__ __launch_bounds__(kT) void split_grad_join(Tile t, const float* __restrict__ parts, const float* __restrict__ weight,
-                                                      float* __restrict__ sums, float* __restrict__ s12) {
-    const size_t unit = size_t(blockIdx.x) * kWaves + (threadIdx.x >> 6);
-    const unsigned lane = threadIdx.x & 63;
-    if (unit >= t.samples * t.groups) return;
-    const size_t n = unit / t.groups, g = unit % t.groups;
-    float s1 = 0.0f, s2 = 0.0f;
-    for (unsigned c = lane; c < t.width; c += 64) {
-        const size_t ch = g * t.width + c;
-        const float* src = parts + n * t.chunks * 2 * t.channels + ch;
-        float sw = 0.0f, sb = 0.0f;
-        for (unsigned q = 0; q < t.chunks; ++q) {
-            sw += src[size_t(q) * 2 * t.channels];
-            sb += src[(size_t(q) * 2 + 1) * t.channels];
+// The chunks' sums per channel, sums[n][2][C]: 64 columns of one sample to a block, every fourth chunk to a
+// wave, eight loads on their way.
+__global__ __launch_bounds__(kT) void split_grad_join(Tile t, const float* __restrict__ parts, float* __restrict__ sums) {
+    __shared__ float s_part[kWaves][64];
+    const size_t cols = 2 * t.channels, tiles = (cols + 63) / 64, n = blockIdx.x / tiles;
+    const unsigned wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const size_t col = (blockIdx.x % tiles) * 64 + lane;
+    float acc[8] = {};
+    if (col < cols) {
+        const float* src = parts + n * t.chunks * cols + col;
+        unsigned q = wave;
+        for (; q + 7 * kWaves < t.chunks; q += 8 * kWaves) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) acc[u] += src[size_t(q + u * kWaves) * cols];
         }
-        sums[n * 2 * t.channels + ch] = sw;
-        sums[(n * 2 + 1) * t.channels + ch] = sb;
-        const float w = weight ? weight[ch] : 1.0f;
-        s1 += sb * w;
-        s2 += sw * w;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (q + u * kWaves < t.chunks) acc[u] += src[size_t(q + u * kWaves) * cols];
     }
-    s1 = lanes_sum(s1, 64);
-    s2 = lanes_sum(s2, 64);
-    if (lane == 0) {
-        const float whole = float(t.positions * t.width);
-        s12[2 * unit] = s1 / whole;
-        s12[2 * unit + 1] = s2 / whole;
-    }
+    s_part[wave][lane] = ((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7]));
+    __syncthreads();
+    if (wave == 0 && col < cols) sums[n * cols + col] = (s_part[0][lane] + s_part[1][lane]) + (s_part[2][lane] + s_part[3][lane]);
 }
 
-template <int V, int ACT>
+template <int V, int ACT, bool STREAM>
 __global__ __launch_bounds__(kT) void split_grad_apply(Tile t, const float* x, const float* __restrict__ weight, const float* __restrict__ bias,
-                                                       const float* __restrict__ stats, const float* __restrict__ s12, const float* g_out,
+                                                       const float* __restrict__ stats, const float* __restrict__ sums, const float* g_out,
                                                        float* dx, size_t n0) {
+    constexpr int kGradRows = grad_rows(STREAM);
+    __shared__ float s_sum[kT][2];
     const Place p = place<V, kT>(t, blockIdx.x);
+    // s1 and s2 of the block's groups, from their channels' sums
+    const unsigned here = t.pieces > 1 ? 1 : p.cols / (t.width / V);
+    const unsigned lanes = t.join_lanes, lane = threadIdx.x & (lanes - 1);
+    for (unsigned g0 = 0; g0 < here; g0 += kT / lanes) {
+        const unsigned g = g0 + threadIdx.x / lanes;
+        float s1 = 0.0f, s2 = 0.0f;
+        if (g < here)
+            for (unsigned c = lane; c < t.width; c += lanes) {
+                const size_t ch = size_t(p.group0 + g) * t.width + c;
+                const float w = weight ? weight[ch] : 1.0f;
+                s2 += sums[p.n * 2 * t.channels + ch] * w;
+                s1 += sums[(p.n * 2 + 1) * t.channels + ch] * w;
+            }
+        s1 = lanes_sum(s1, int(lanes));
+        s2 = lanes_sum(s2, int(lanes));
+        if (g < here && lane == 0) {
+            const float whole = float(t.positions * t.width);
+            s_sum[g][0] = s1 / whole;
+            s_sum[g][1] = s2 / whole;
+        }
+    }
+    __syncthreads();
     if (!p.live) return;
     const unsigned gl = t.pieces > 1 ? 0 : p.col / (t.width / V);
     const float* st = stats + 2 * ((n0 + p.n) * t.groups + p.group0 + gl);
     const float mean = st[0], rstd = st[1];
-    const float* ss = s12 + 2 * (p.n * t.groups + p.group0 + gl);
-    const float s1 = ss[0], s2 = ss[1];
+    const float s1 = s_sum[gl][0], s2 = s_sum[gl][1];
     const Vec<V> w = affine_vec<V>(weight, p.col0 + p.col * V, 1.0f), b = affine_vec<V>(bias, p.col0 + p.col * V, 0.0f);
     size_t at = ((n0 + p.n) * t.positions + p.first + p.row) * t.channels + p.col0 + p.col * V;
     const size_t step = size_t(t.row_lanes) * t.channels;
     size_t left = rows_of(p.first + p.row, p.last, t.row_lanes);
-    for (; left > 0; at += kGradRows * step) {
-        const int count = left < kGradRows ? int(left) : kGradRows;
+    auto batch = [&](auto full) {
+        const int count = decltype(full)::value ? kGradRows : int(left);
         Vec<V> h[kGradRows], d[kGradRows];
 #pragma unroll
         for (int k = 0; k < kGradRows; ++k) {
-            h[k] = k < count ? load_vec<V>(x + at + k * step) : Vec<V>{};
-            d[k] = k < count ? load_vec<V>(g_out + at + k * step) : Vec<V>{};
+            h[k] = k < count ? load_vec<V, STREAM>(x + at + k * step) : Vec<V>{};
+            d[k] = k < count ? load_vec<V, STREAM>(g_out + at + k * step) : Vec<V>{};
         }
 #pragma unroll
         for (int k = 0; k < kGradRows; ++k)
@@ -725,36 +794,45 @@ __global__ __launch_bounds__(kT) void split_grad_apply(Tile t, const float* x, c
                 }
                 store_vec<V>(dx + at + k * step, o);
             }
-        left -= count;
-    }
+    };
+    for (; left >= kGradRows; at += kGradRows * step, left -= kGradRows) batch(std::true_type{});
+    if (left > 0) batch(std::false_type{});
 }
 
-// dweight[c] (+)= sum of partials[r][0][c], dbias likewise from [r][1][c], r in a fixed order: 16 threads
-// take every 16th row of 16 columns, then add through LDS.
-__global__ __launch_bounds__(kT) void grad_columns(const float* __restrict__ partials, size_t rows, size_t channels, float* __restrict__ dweight,
-                                                   float* __restrict__ dbias, int add) {
-    __shared__ float s_part[16][17];
+// dweight[c] (+)= sum of partials[r][0][c], dbias likewise from [r][1][c], r in a fixed order: 64 threads
+// take every 64th row of 16 columns, four on their way, then add through LDS.
+constexpr unsigned kFoldThreads = 1024;
+__global__ __launch_bounds__(kFoldThreads) void grad_columns(const float* __restrict__ partials, size_t rows, size_t channels,
+                                                             float* __restrict__ dweight, float* __restrict__ dbias, int add) {
+    __shared__ float s_part[64][17];
     const unsigned c = threadIdx.x & 15, r0 = threadIdx.x >> 4;
     const size_t col = size_t(blockIdx.x) * 16 + c, cols = 2 * channels;
     float acc[4] = {};
     if (col < cols) {
         size_t r = r0;
-        for (; r + 48 < rows; r += 64) {
+        for (; r + 192 < rows; r += 256) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) acc[q] += partials[(r + 16 * q) * cols + col];
+            for (int q = 0; q < 4; ++q) acc[q] += partials[(r + 64 * q) * cols + col];
         }
-        for (; r < rows; r += 16) acc[0] += partials[r * cols + col];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (r + 64 * q < rows) acc[q] += partials[(r + 64 * q) * cols + col];
     }
     s_part[r0][c] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
     __syncthreads();
-    if (threadIdx.x < 16 && col < cols) {
+    if (threadIdx.x < 64) {                           // 4 threads to a column, 16 rows each
+        const unsigned part = threadIdx.x >> 4;
         float s = 0.0f;
 #pragma unroll
-        for (int q = 0; q < 16; ++q) s += s_part[q][c];
-        float* out = col < channels ? dweight : dbias;
-        if (out) {
-            float* o = out + (col < channels ? col : col - channels);
-            *o = add ? *o + s : s;
+        for (int q = 0; q < 16; ++q) s += s_part[part * 16 + q][c];
+        s += __shfl_xor(s, 16, 64);
+        s += __shfl_xor(s, 32, 64);
+        if (part == 0 && col < cols) {
+            float* out = col < channels ? dweight : dbias;
+            if (out) {
+                float* o = out + (col < channels ? col : col - channels);
+                *o = add ? *o + s : s;
+            }
         }
     }
 }
@@ -778,9 +856,8 @@ unsigned vector_width(size_t width, std::initializer_list<const void*> ptrs) {
 constexpr unsigned kRowVectors = 8;             // most vectors a lane holds in the rows kernels
 bool rows_fit(size_t positions, size_t width, unsigned v) { return positions == 1 && width / v <= 64 * kRowVectors; }
 
-// The smallest run of whole groups that fills a 128-byte line in every row, so that a block does not
-// fetch lines it uses a part of - or the whole row, if that is shorter.
-Tile tile_of(size_t n, size_t s, size_t c, unsigned groups, unsigned v, unsigned threads, bool whole_lines_only) {
+// `least` groups to a block, or as many as fill its threads once (least == 0).
+Tile tile_of(size_t n, size_t s, size_t c, unsigned groups, unsigned v, unsigned threads, unsigned least) {
     Tile t{};
     t.samples = n;
     t.positions = s;
@@ -797,25 +874,38 @@ Tile tile_of(size_t n, size_t s, size_t c, unsigned groups, unsigned v, unsigned
     } else {
         t.pieces = 1;
         unsigned bg = threads / wv;
-        if (whole_lines_only) {
-            const unsigned want = (32 + t.width - 1) / t.width;
-            if (want < bg) bg = want;
-        }
+        if (least && least < bg) bg = least;
         if (bg > groups) bg = groups;
         t.block_groups = bg;
         t.cols = bg * wv;
         t.col_blocks = (groups + bg - 1) / bg;
     }
     t.row_lanes = threads / t.cols;
+    const unsigned lanes = pow2_at_least(threads / t.block_groups / 2 + 1);         // the power of two at most threads / block_groups
+    t.join_lanes = lanes < 64 ? lanes : 64;
     t.chunks = 1;
     t.chunk_rows = s;
     return t;
 }
 
+// The run of whole groups that a block of `threads` keeps in registers, at most `most` vectors a thread: as
+// many groups as fill a 128-byte line in every row, so that a block does not fetch lines it uses a part of -
+// or all, if that is less.  (16 x 4096 x 256 in groups of 8 channels, one group to a block of 1024: 51.7 us
+// from HBM, with neighbours on one XCD; the split form takes 44.2.)
+bool resident_tile(Tile* t, size_t n, size_t s, size_t c, unsigned groups, unsigned v, unsigned threads, size_t most, size_t* held) {
+    const unsigned width = unsigned(c / groups);
+    *t = tile_of(n, s, c, groups, v, threads, (32 + width - 1) / width);
+    *held = (s + t->row_lanes - 1) / t->row_lanes;
+    return t->pieces == 1 && *held <= most;
+}
+
+// two blocks to a CU: their loads fill it, and the parts to join stay few (5 x 7031 x 330 forward and backward
+// 30.9 and 44.7 us; eight 32.8 and 50.0)
+constexpr size_t kBlocksPerCu = 2;
 // Positions per block of the split kernels: enough blocks for the chip, at least 32 rows of work each
 void split_positions(Tile* t, size_t per_part_floats, size_t floats) {
     const size_t cus = size_t(compute_units() > 0 ? compute_units() : 256);
-    const size_t want = 8 * cus, others = t->samples * t->col_blocks;
+    const size_t want = kBlocksPerCu * cus, others = t->samples * t->col_blocks;
     size_t chunks = others >= want ? 1 : (want + others - 1) / others;
     const size_t most = (t->positions + size_t(t->row_lanes) * 16 - 1) / (size_t(t->row_lanes) * 16);
     if (chunks > most) chunks = most;
@@ -826,6 +916,11 @@ void split_positions(Tile* t, size_t per_part_floats, size_t floats) {
     t->chunks = unsigned((t->positions + t->chunk_rows - 1) / t->chunk_rows);
 }
 
+#define BY_STREAM(YES, ...)                                                        \
+    do {                                                                           \
+        if (YES) { constexpr bool STREAM = true; __VA_ARGS__; }                    \
+        else { constexpr bool STREAM = false; __VA_ARGS__; }                       \
+    } while (0)
 #define BY_ACT(ACT_VALUE, ...)                                                     \
     do {                                                                           \
         if ((ACT_VALUE) == CTAMD_ACT_RELU) { constexpr int ACT = CTAMD_ACT_RELU; __VA_ARGS__; } \
@@ -846,8 +941,15 @@ void split_positions(Tile* t, size_t per_part_floats, size_t floats) {
         else { constexpr int K = 8; __VA_ARGS__; }                                 \
     } while (0)
 
+// Whether what the first launch of the split form reads has left the memory-side cache (256 MiB) before
+// the last one reads it again: then both read with the streaming hint, which leaves the cache to the result
+// (forward / backward with the hint and without: 128 MiB read 74 / 69 us and 70 / 64 us, 256 MiB 130 / 122
+// and 167 / 139 us, 512 MiB 298 / 234 and 324 / 285 us).
+bool input_streams(double floats) { return floats * 4.0 > 160.0 * 1024 * 1024; }
+
 // Blocks per launch (1024 threads each stay below 2^32); longer batches take several launches.  2^20
 // channels at most, so that one sample's blocks always fit, and its sums fit the scratch.
+constexpr unsigned kInlineParts = 64;           // parts of a group that every block of the last launch joins for itself (a launch less, 3 us)
 constexpr size_t kMostBlocks = size_t(1) << 21;
 constexpr size_t kMostChannels = size_t(1) << 20;
 
@@ -892,9 +994,9 @@ int ctamd_group_norm_f32(const float* x, const float* weight, const float* bias,
         return CTAMD_OK;
     }
     for (unsigned threads : {256u, 1024u}) {
-        const Tile t = tile_of(batch, positions, channels, unsigned(groups), v, threads, true);
-        const size_t held = (positions + t.row_lanes - 1) / t.row_lanes;
-        if (t.pieces > 1 || held > 8) continue;
+        Tile t;
+        size_t held;
+        if (!resident_tile(&t, batch, positions, channels, unsigned(groups), v, threads, 8, &held)) continue;
         const size_t slab = kMostBlocks / t.col_blocks;
         for (size_t n0 = 0; n0 < batch; n0 += slab) {
             const size_t samples = batch - n0 < slab ? batch - n0 : slab;
@@ -918,7 +1020,8 @@ int ctamd_group_norm_f32(const float* x, const float* weight, const float* bias,
     float* scratch = use.ptr();
     if (!scratch) return CTAMD_EINVAL;
     // samples at a time: as many as leave room for a (mean, M2) pair per part and the joined statistics
-    Tile t = tile_of(batch, positions, channels, unsigned(groups), v, kT, false);
+    const bool stream_in = input_streams(elements);
+    Tile t = tile_of(batch, positions, channels, unsigned(groups), v, kT, 0);
     const size_t per_sample = 2 * groups * (t.pieces + 1);
     size_t slab = kScratchFloats / per_sample;
     if (slab > kMostBlocks / t.col_blocks) slab = kMostBlocks / t.col_blocks;
@@ -932,13 +1035,17 @@ int ctamd_group_norm_f32(const float* x, const float* weight, const float* bias,
         float* ys = y + n0 * positions * channels;
         float* st = stats ? stats + 2 * n0 * groups : scratch;
         float* parts = scratch + 2 * units;
-        BY_VEC(v, hipLaunchKernelGGL((split_stats<V>), dim3(unsigned(blocks)), dim3(kT), 0, s, t, xs, parts));
+        BY_VEC(v, BY_STREAM(stream_in, hipLaunchKernelGGL((split_stats<V, STREAM>), dim3(unsigned(blocks)), dim3(kT), 0, s, t, xs, parts)));
         rc = launched(__func__);
         if (rc) return rc;
-        BY_VEC(v, hipLaunchKernelGGL((split_join<V>), dim3(unsigned((units + kWaves - 1) / kWaves)), dim3(kT), 0, s, t, parts, eps, st));
-        rc = launched(__func__);
-        if (rc) return rc;
-        BY_VEC(v, BY_ACT(act, hipLaunchKernelGGL((split_apply<V, ACT>), dim3(unsigned(blocks)), dim3(kT), 0, s, t, xs, weight, bias, st, ys)));
+        const bool inline_join = size_t(t.pieces) * t.chunks <= kInlineParts;
+        if (!inline_join) {
+            BY_VEC(v, hipLaunchKernelGGL((split_join<V>), dim3(unsigned((units + kWaves - 1) / kWaves)), dim3(kT), 0, s, t, parts, eps, st));
+            rc = launched(__func__);
+            if (rc) return rc;
+        }
+        BY_VEC(v, BY_ACT(act, BY_STREAM(stream_in, hipLaunchKernelGGL((split_apply<V, ACT, STREAM>), dim3(unsigned(blocks)), dim3(kT), 0, s, t, xs, weight,
+                                                                      bias, st, inline_join ? parts : nullptr, eps, ys))));
         rc = launched(__func__);
         if (rc) return rc;
     }
@@ -967,14 +1074,14 @@ int ctamd_group_norm_backward_f32(const float* x, const float* weight, const flo
     if (!scratch) return CTAMD_EINVAL;
     const size_t most_rows = kScratchFloats / (2 * channels);           // rows of partial sums that the scratch holds (at least 2)
     auto fold = [&](const float* partials, size_t rows, int add) {
-        hipLaunchKernelGGL(grad_columns, dim3(unsigned((2 * channels + 15) / 16)), dim3(kT), 0, s, partials, rows, channels, dweight, dbias, add);
+        hipLaunchKernelGGL(grad_columns, dim3(unsigned((2 * channels + 15) / 16)), dim3(kFoldThreads), 0, s, partials, rows, channels, dweight, dbias, add);
         return launched("ctamd_group_norm_backward_f32");
     };
     if (rows_fit(positions, width, v)) {
         const unsigned wv = unsigned(width / v), lanes = pow2_at_least(wv < 64 ? wv : 64), count = (wv + lanes - 1) / lanes;
         const unsigned subs = kT / lanes, block_groups = groups < subs ? unsigned(groups) : subs, sample_lanes = subs / block_groups;
         const size_t col_blocks = (groups + block_groups - 1) / block_groups;
-        size_t blocks = (batch + sample_lanes - 1) / sample_lanes, want = 4 * cus / col_blocks;
+        size_t blocks = (batch + sample_lanes - 1) / sample_lanes, want = 2 * cus / col_blocks;
         if (want < 1) want = 1;
         if (blocks > want) blocks = want;
         if (blocks > most_rows) blocks = most_rows;
@@ -988,9 +1095,9 @@ int ctamd_group_norm_backward_f32(const float* x, const float* weight, const flo
         return rc;
     }
     for (unsigned threads : {256u, 1024u}) {
-        const Tile t = tile_of(batch, positions, channels, unsigned(groups), v, threads, true);
-        const size_t held = (positions + t.row_lanes - 1) / t.row_lanes;
-        if (t.pieces > 1 || held > (threads == 256 ? 8 : 4)) continue;
+        Tile t;
+        size_t held;
+        if (!resident_tile(&t, batch, positions, channels, unsigned(groups), v, threads, threads == 256 ? 8 : 4, &held)) continue;
         size_t rows = 4 * cus * 256 / threads / t.col_blocks;
         if (rows < 1) rows = 1;
         if (rows > batch) rows = batch;
@@ -1012,28 +1119,29 @@ int ctamd_group_norm_backward_f32(const float* x, const float* weight, const flo
         if (!rc) account(12.0 * elements, 16.0 * elements);
         return rc;
     }
-    Tile t = tile_of(batch, positions, channels, unsigned(groups), v, kT, false);
-    // per sample: its channels' sums, s1 and s2 per group, and one part at least
-    const size_t per_sample = 2 * channels + 2 * groups;
+    const bool stream_in = input_streams(2.0 * elements);
+    Tile t = tile_of(batch, positions, channels, unsigned(groups), v, kT, 0);
+    // per sample: its channels' sums, and one part at least
+    const size_t per_sample = 2 * channels;
     size_t slab = kScratchFloats / (per_sample + 2 * channels);
     if (slab > kMostBlocks / t.col_blocks) slab = kMostBlocks / t.col_blocks;
     if (slab > batch) slab = batch;
     for (size_t n0 = 0; n0 < batch; n0 += slab) {
         t.samples = batch - n0 < slab ? batch - n0 : slab;
         split_positions(&t, 2 * channels * t.samples, kScratchFloats - t.samples * per_sample);
-        const size_t blocks = t.samples * t.col_blocks * t.chunks, units = t.samples * groups;
+        const size_t blocks = t.samples * t.col_blocks * t.chunks;
         float* sums = scratch;
-        float* s12 = sums + t.samples * 2 * channels;
-        float* parts = s12 + 2 * units;
-        BY_VEC(v, BY_ACT(act, hipLaunchKernelGGL((split_grad_sums<V, ACT>), dim3(unsigned(blocks)), dim3(kT), 0, s, t, x, weight, bias, stats, g, parts, n0)));
+        float* parts = sums + t.samples * 2 * channels;
+        BY_VEC(v, BY_ACT(act, BY_STREAM(stream_in, hipLaunchKernelGGL((split_grad_sums<V, ACT, STREAM>), dim3(unsigned(blocks)), dim3(kT), 0, s, t, x, weight,
+                                                                      bias, stats, g, parts, n0))));
         rc = launched(__func__);
         if (rc) return rc;
-        hipLaunchKernelGGL(split_grad_join, dim3(unsigned((units + kWaves - 1) / kWaves)), dim3(kT), 0, s, t, parts, weight, sums, s12);
+        hipLaunchKernelGGL(split_grad_join, dim3(unsigned(t.samples * ((2 * channels + 63) / 64))), dim3(kT), 0, s, t, parts, sums);
         rc = launched(__func__);
         if (rc) return rc;
         if (dx) {
-            BY_VEC(v, BY_ACT(act, hipLaunchKernelGGL((split_grad_apply<V, ACT>), dim3(unsigned(blocks)), dim3(kT), 0, s, t, x, weight, bias, stats, s12, g,
-                                                     dx, n0)));
+            BY_VEC(v, BY_ACT(act, BY_STREAM(stream_in, hipLaunchKernelGGL((split_grad_apply<V, ACT, STREAM>), dim3(unsigned(blocks)), dim3(kT), 0, s, t, x,
+                                                                          weight, bias, stats, sums, g, dx, n0))));
             rc = launched(__func__);
             if (rc) return rc;
         }
