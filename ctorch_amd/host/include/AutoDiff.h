@@ -66,6 +66,12 @@ class AutoDiff {
         Tensor index;    // max / min: position of the extreme element along the axis (int32)
         Tensor mean;     // var / std
     };
+    // a group normalisation (op::GroupNorm): its shape and the statistics that the forward pass left
+    struct GroupNormPayload : OpPayload {
+        size_t groups = 1;
+        Activation act = Activation::kNone;
+        Tensor stats;
+    };
     // what Tensor::linear_cross_entropy formed in its one pass (op::LinearCE): the gradient of the logits
     // for an upstream gradient of 1, and from it the gradients of the three inputs
     struct LinearCEPayload : OpPayload {

@@ -27,6 +27,7 @@ enum class op {
     // have no enumerator there because nothing tapes them
     Abs, Exp, Log, Sqrt, Square, Tan, LogSoftmax,
     Reduce,   // sum / mean / max / min / var / std along dimensions; which one is in the node's payload
+    GroupNorm, // not in the reference: normalisation over groups of channels with an activation, Tensor::group_norm
 };
 
 enum class ErrorLevel { TRACE = 0, DEBUG = 1, INFO = 2, WARN = 3, ERROR = 4, FATAL = 5 };

@@ -25,6 +25,9 @@
 
 struct ShapeTag {};
 
+// what Tensor::group_norm applies to its result (the CTAMD_ACT_* codes)
+enum class Activation { kNone = 0, kReLU = 1, kSiLU = 2 };
+
 class Tensor {
    private:
     size_t tensor_id_;
@@ -152,6 +155,12 @@ class Tensor {
     // where the two-operator form's logits node would accumulate too.  Any other shape, a host tensor or
     // one-hot targets: the two operators.  logits (optional) receives x.linear(weight, bias).
     Tensor linear_cross_entropy(const Tensor& weight, const Tensor& bias, const Tensor& labels, Tensor* logits = nullptr) const;
+    // Not in the reference: group normalisation of a channels-last tensor [samples, ..., channels] (2-D: a
+    // layer's activations, one position per sample) with an activation, as one operator and one tape
+    // entry: act((x - mean) * rstd * weight + bias), mean and rstd over each sample's positions and each of
+    // `groups` equal runs of channels; weight and bias are [channels].  groups = 1 on a 2-D tensor is
+    // layer normalisation.  Gradients of all three operands come from one call.
+    Tensor group_norm(size_t groups, const Tensor& weight, const Tensor& bias, Activation act = Activation::kNone, float eps = 1e-5f) const;
     Tensor dot(const Tensor& other) const;
     Tensor relu() const;
     Tensor sigmoid() const;

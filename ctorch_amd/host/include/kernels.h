@@ -91,6 +91,10 @@ bool ce_one_pass();
 // tensors that are not fp32 (the typed arms of src/Tensor.cpp:197-243, :390-448)
 void fill_typed(void* device_ptr, DType dtype, double v, size_t n);    // zero() / ones() of any dtype, device memory
 Tensor cast_from_float(const Tensor& a, DType to);                    // Tensor::to(DType)
+// group normalisation with an activation, and its gradients (those of the three that are not null)
+Tensor group_norm(const Tensor& x, size_t groups, const Tensor& weight, const Tensor& bias, Activation act, float eps, Tensor* stats);
+void group_norm_backward(const Tensor& x, size_t groups, const Tensor& weight, const Tensor& bias, Activation act, const Tensor& stats,
+                         const Tensor& g, Tensor* dx, Tensor* dweight, Tensor* dbias);
 Tensor softmax_dim(const Tensor& a, int dim);                         // dim already normalised
 Tensor filled(const std::vector<size_t>& shape, float v, DeviceType device);
 void fill_scalar(Tensor& t, float v);                                  // every element of a device tensor = v
@@ -108,6 +112,16 @@ void sgd_step(Tensor& param, const Tensor& grad, float lr);            // mnist/
 // the same update for several parameters in one launch; grads as AutoDiff::stored_grad returns them
 // (an empty gradient leaves its parameter alone), "0 +" applied in the kernel
 void sgd_step_all(const std::vector<Tensor*>& params, const std::vector<Tensor>& grads, float lr);
+// Not in the reference: the orthogonalised update of several 2-D parameters in one call, in place
+// (ctamd_muon_step_f32: momentum, Newton-Schulz iteration, weight decay).  grads as
+// AutoDiff::stored_grad returns them (an empty gradient leaves its parameter alone), momenta of the
+// parameters' shapes, zeros at the start.  The update is 0.2 * sqrt(max(rows, cols)) times the
+// orthogonalised matrix: about as large, element by element, as an adaptive optimiser's.
+void muon_step_all(const std::vector<Tensor*>& params, const std::vector<Tensor>& grads, const std::vector<Tensor*>& momenta, float lr,
+                   float momentum = 0.95f, bool nesterov = true, float weight_decay = 0.0f, int steps = 5);
+// g [rows, cols], or [batch, rows, cols] matrix by matrix, with its singular values driven towards one
+// (ctamd_newton_schulz_f32 with its own coefficients)
+Tensor newton_schulz(const Tensor& g, int steps = 5);
 size_t count_correct(const Tensor& pred, const Tensor& labels);        // mnist/mnist.cpp:134-156 (reads back)
 Tensor unit_from_bytes(const unsigned char* host_bytes, size_t rows, size_t cols);  // mnist_loader.cpp:33-41
 Tensor relu_backward(const Tensor& x, const Tensor& g);

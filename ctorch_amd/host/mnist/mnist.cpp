@@ -3,9 +3,13 @@
 //
 //   mnist.bin [--data DIR] [--epochs N] [--batch N] [--lr X] [--hidden1 N] [--hidden2 N]
 //             [--reference-tape | --graph] [--fused | --fused-head] [--loss-each-step]
+//             [--norm GROUPS] [--muon RATE]
 //
 // --graph records one training step into a HIP graph at the first batch and replays it for every
 // batch: one launch per step instead of about fifty.
+//
+// --norm normalises the hidden layers over groups of units before their ReLU; --muon updates the weight
+// matrices by their orthogonalised momentum (0.02 is a usual rate), the other parameters by SGD with --lr.
 //
 // --reference-tape reproduces two properties of the reference's tape that change the numbers:
 // bias gradients taken from row 0 of the upstream gradient, and leaf values frozen at their
@@ -36,6 +40,8 @@ int main(int argc, char** argv) {
         else if (a == "--fused") opt.fused_layers = true;
         else if (a == "--fused-head") opt.fused_layers = opt.fused_head = true;
         else if (a == "--loss-each-step") opt.loss_on_device = false;
+        else if (a == "--norm") opt.norm_groups = std::atoi(next());
+        else if (a == "--muon") opt.muon_rate = float(std::atof(next()));
         else {
             std::fprintf(stderr, "unknown option %s\n", a.c_str());
             return 2;

@@ -34,6 +34,10 @@ struct MnistDemoOptions {
     // false: every step reads its loss, as the reference's loop does for its progress line
     // (mnist/mnist.cpp:253-260).
     bool loss_on_device = true;
+    // not in the reference: the hidden layers normalised over this many groups of units (0: not), and the
+    // weight matrices updated by their orthogonalised momentum with this rate (0: plain SGD)
+    int norm_groups = 0;
+    float muon_rate = 0.0f;
 };
 
 struct MnistDemoResult {
@@ -61,6 +65,8 @@ inline MnistDemoResult run_mnist_demo(const MnistDemoOptions& opt) {
     NeuralNetwork model(int(res.pixels), opt.hidden1, opt.hidden2, 10, opt.learning_rate);
     model.fused_layers = opt.fused_layers;
     model.fused_head = opt.fused_head;
+    if (opt.norm_groups > 0) model.normalise(size_t(opt.norm_groups));
+    if (opt.muon_rate != 0.0f) model.use_muon(opt.muon_rate);
     res.num_batches = int(res.train_images) / opt.batch_size;
 
     AutoDiff autodiff;

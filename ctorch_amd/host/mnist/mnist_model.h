@@ -17,6 +17,10 @@
 class NeuralNetwork {
    public:
     Tensor W1, b1, W2, b2, W3, b3;
+    // with normalise(): weight and bias of the hidden layers' normalisation
+    Tensor n1w, n1b, n2w, n2b;
+    // with use_muon(): the weight matrices' momenta
+    Tensor m1, m2, m3;
     float learning_rate;
 
     // Weights uniform in +-sqrt(1/fan_in) from the C library's rand() in the reference's order
@@ -48,10 +52,45 @@ class NeuralNetwork {
     // within the MatMul bound of the other forms
     bool fused_head = false;
 
-    Tensor forward(const Tensor& x) {
-        if (fused_layers) return x.linear(W1, b1, true).linear(W2, b2, true).linear(W3, b3, false);
+    // Not in the reference: each hidden layer is x.W + b, normalised over `groups` runs of its units, then
+    // ReLU (Tensor::group_norm); weights start at one, biases at zero, and all are trained.
+    void normalise(size_t groups) {
+        norm_groups = groups;
+        n1w = ctorch_amd_host::filled({W1.sizes()[1]}, 1.0f, DeviceType::kAMD);
+        n1b = ctorch_amd_host::filled({W1.sizes()[1]}, 0.0f, DeviceType::kAMD);
+        n2w = ctorch_amd_host::filled({W2.sizes()[1]}, 1.0f, DeviceType::kAMD);
+        n2b = ctorch_amd_host::filled({W2.sizes()[1]}, 0.0f, DeviceType::kAMD);
+    }
+    size_t norm_groups = 0;
+    // Not in the reference: the three weight matrices are updated by their orthogonalised momentum
+    // (ctorch_amd_host::muon_step_all) with a rate of their own, everything else by plain SGD.
+    void use_muon(float lr) {
+        muon_rate = lr;
+        m1 = ctorch_amd_host::filled(W1.sizes(), 0.0f, DeviceType::kAMD);
+        m2 = ctorch_amd_host::filled(W2.sizes(), 0.0f, DeviceType::kAMD);
+        m3 = ctorch_amd_host::filled(W3.sizes(), 0.0f, DeviceType::kAMD);
+    }
+    float muon_rate = 0.0f;
+
+    // the hidden activations that the last layer reads
+    Tensor hidden(const Tensor& x) {
+        if (norm_groups) {
+            if (fused_layers)
+                return x.linear(W1, b1, false).group_norm(norm_groups, n1w, n1b, Activation::kReLU).linear(W2, b2, false).group_norm(
+                    norm_groups, n2w, n2b, Activation::kReLU);
+            Tensor z1 = x.matmul(W1) + b1;
+            Tensor h1 = z1.group_norm(norm_groups, n1w, n1b, Activation::kReLU);
+            Tensor z2 = h1.matmul(W2) + b2;
+            return z2.group_norm(norm_groups, n2w, n2b, Activation::kReLU);
+        }
+        if (fused_layers) return x.linear(W1, b1, true).linear(W2, b2, true);
         Tensor h1 = (x.matmul(W1) + b1).relu();
-        Tensor h2 = (h1.matmul(W2) + b2).relu();
+        return (h1.matmul(W2) + b2).relu();
+    }
+
+    Tensor forward(const Tensor& x) {
+        if (fused_layers) return hidden(x).linear(W3, b3, false);
+        Tensor h2 = hidden(x);
         return h2.matmul(W3) + b3;
     }
 
@@ -63,7 +102,7 @@ class NeuralNetwork {
     // forward and backward, mnist/mnist.cpp:80-81; the value is the same wherever it is read.)
     Tensor train_step_on_device(const Tensor& x, const Tensor& y) {
         AutoDiff* ctx = AutoDiffContext::current();
-        Tensor* params[6] = {&W1, &b1, &W2, &b2, &W3, &b3};
+        const std::vector<Tensor*> params = parameters();
         if (ctx)
             for (Tensor* p : params) ctx->make_leaf(*p, true);
         for (Tensor* p : params) p->requires_grad(true);
@@ -71,7 +110,7 @@ class NeuralNetwork {
             for (Tensor* p : params) ctx->zero_grad(*p);
         Tensor loss;
         if (fused_layers && fused_head) {
-            loss = x.linear(W1, b1, true).linear(W2, b2, true).linear_cross_entropy(W3, b3, y);
+            loss = hidden(x).linear_cross_entropy(W3, b3, y);
         } else {
             Tensor logits = forward(x);
             Tensor y_one_hot = ctorch_amd_host::onehot(y, logits.sizes()[1]);
@@ -82,14 +121,27 @@ class NeuralNetwork {
         return loss;
     }
 
+    std::vector<Tensor*> parameters() {
+        std::vector<Tensor*> ps{&W1, &b1, &W2, &b2, &W3, &b3};
+        if (norm_groups) ps.insert(ps.end(), {&n1w, &n1b, &n2w, &n2b});
+        return ps;
+    }
+
     void update_parameters() {
-        Tensor* params[6] = {&W1, &b1, &W2, &b2, &W3, &b3};
+        std::vector<Tensor*> params = parameters();
         AutoDiff* ctx = AutoDiffContext::current();
-        if (fused_layers && ctx) {                       // one launch for the six tensors
-            std::vector<Tensor*> ps(params, params + 6);
+        if (muon_rate != 0.0f && ctx) {
+            std::vector<Tensor*> matrices{&W1, &W2, &W3}, momenta{&m1, &m2, &m3};
+            std::vector<Tensor> gs;
+            for (Tensor* p : matrices) gs.push_back(ctx->stored_grad(*p));
+            ctorch_amd_host::muon_step_all(matrices, gs, momenta, muon_rate);
+            params = {&b1, &b2, &b3};
+            if (norm_groups) params.insert(params.end(), {&n1w, &n1b, &n2w, &n2b});
+        }
+        if (fused_layers && ctx) {                       // one launch for all the tensors
             std::vector<Tensor> gs;
             for (Tensor* p : params) gs.push_back(ctx->stored_grad(*p));
-            ctorch_amd_host::sgd_step_all(ps, gs, learning_rate);
+            ctorch_amd_host::sgd_step_all(params, gs, learning_rate);
             return;
         }
         for (Tensor* p : params) {

@@ -409,6 +409,21 @@ Tensor AutoDiff::input_gradient(Node* node, size_t input_id, size_t input_pos, c
             term_plus_zero_ = false;
             return Tensor::alias(gz);                                   // shaped by the caller (column sums, or row 0)
         }
+        case op::GroupNorm: {
+            if (node->input_grads.empty()) {
+                auto* kept = dynamic_cast<GroupNormPayload*>(node->payload.get());
+                if (!kept)
+                    Ctorch_Error::throwException(ErrorPlatform::kAutoDiff, ErrorType::TENSOR_STATE, "backward: group norm without its record");
+                Node* in[3] = {find(node->input_ids[0]), find(node->input_ids[1]), find(node->input_ids[2])};
+                node->input_grads.resize(3);
+                Tensor* want[3];
+                for (int i = 0; i < 3; ++i) want[i] = in[i]->requires_grad ? &node->input_grads[i] : nullptr;
+                Tensor up = g.sizes() == in[0]->tensor->sizes() ? Tensor::alias(g) : adjust_grad_shape(g, in[0]->tensor->sizes());
+                group_norm_backward(*in[0]->tensor, kept->groups, *in[1]->tensor, *in[2]->tensor, kept->act, kept->stats, up, want[0], want[1], want[2]);
+            }
+            term_plus_zero_ = input_pos != 0;                           // sums that start from +0; x's gradient may hold -0
+            return Tensor::alias(node->input_grads[input_pos]);
+        }
         case op::Fused: {                                               // every operator branch above, in one launch
             if (node->input_grads.empty()) {
                 auto* program = dynamic_cast<FusedPayload*>(node->payload.get());

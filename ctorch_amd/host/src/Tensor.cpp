@@ -380,6 +380,19 @@ Tensor Tensor::linear_cross_entropy(const Tensor& weight, const Tensor& bias, co
     if (taped) tape(result, op::LinearCE, {this, &weight, &bias}, 0, kept);
     return result;
 }
+Tensor Tensor::group_norm(size_t groups, const Tensor& weight, const Tensor& bias, Activation act, float eps) const {
+    if (device() != DeviceType::kAMD)
+        Ctorch_Error::throwException(ErrorPlatform::kGENERAL, ErrorType::PLATFORM_API, "group_norm: no kernel for this device");
+    check_pair(*this, weight);
+    check_pair(*this, bias);
+    const bool taped = AutoDiffContext::current() && (requires_grad() || weight.requires_grad() || bias.requires_grad());
+    auto kept = std::make_shared<AutoDiff::GroupNormPayload>();
+    kept->groups = groups;
+    kept->act = act;
+    Tensor result = ctorch_amd_host::group_norm(*this, groups, weight, bias, act, eps, taped ? &kept->stats : nullptr);
+    tape(result, op::GroupNorm, {this, &weight, &bias}, 0, kept);
+    return result;
+}
 namespace {
 Tensor compare_with(int cmp, const Tensor& a, const Tensor* b, float s) {
     if (a.device() != DeviceType::kAMD)

@@ -5,6 +5,8 @@
 // label-range flag).
 #include "kernels.h"
 
+#include <cmath>
+
 #include "AutoDiff.h"
 
 #include "ctorch_amd.h"
@@ -195,6 +197,50 @@ Tensor compare_op(int cmp, const Tensor& a, const Tensor* b, float s) {
           : ctamd_compare_scalar_f32(cmp, a.fptr(), s, out, a.numel(), current_stream()),
         "comparison");
     return r;
+}
+namespace {
+// samples, positions and channels of a channels-last tensor
+void channels_last(const Tensor& x, size_t& samples, size_t& positions, size_t& channels, const char* who) {
+    if (x.dim() < 2 || !x.is_contiguous())
+        Ctorch_Error::throwException(kP, ErrorType::DIMENSION, std::string(who) + ": a contiguous tensor [samples, ..., channels] is needed");
+    samples = x.sizes().front();
+    channels = x.sizes().back();
+    positions = 1;
+    for (size_t d = 1; d + 1 < x.dim(); ++d) positions *= x.sizes()[d];
+}
+void check_per_channel(const Tensor& t, size_t channels, const char* who) {
+    check_device(t, who);
+    if (t.dim() != 1 || t.sizes()[0] != channels || !t.is_contiguous())
+        Ctorch_Error::throwException(kP, ErrorType::DIMENSION, std::string(who) + ": weight and bias are [channels]");
+}
+}  // namespace
+Tensor group_norm(const Tensor& x, size_t groups, const Tensor& weight, const Tensor& bias, Activation act, float eps, Tensor* stats) {
+    check_device(x, "group_norm");
+    size_t n = 0, p = 0, c = 0;
+    channels_last(x, n, p, c, "group_norm");
+    check_per_channel(weight, c, "group_norm");
+    check_per_channel(bias, c, "group_norm");
+    Tensor r = like(x);
+    if (stats) *stats = Tensor(ShapeTag{}, {n, groups, 2}, DType::kFloat, DeviceType::kAMD, false);
+    run(ctamd_group_norm_f32(x.fptr(), weight.fptr(), bias.fptr(), eps, int(act), r.fptr(), stats ? stats->fptr() : nullptr, n, p, c, groups,
+                             current_stream()),
+        "group_norm");
+    return r;
+}
+void group_norm_backward(const Tensor& x, size_t groups, const Tensor& weight, const Tensor& bias, Activation act, const Tensor& stats, const Tensor& g,
+                         Tensor* dx, Tensor* dweight, Tensor* dbias) {
+    check_device(x, "group_norm gradient");
+    check_device(g, "group_norm gradient");
+    size_t n = 0, p = 0, c = 0;
+    channels_last(x, n, p, c, "group_norm gradient");
+    if (g.sizes() != x.sizes() || !g.is_contiguous())
+        Ctorch_Error::throwException(kP, ErrorType::DIMENSION, "group_norm gradient: sizes differ");
+    if (dx) *dx = like(x);
+    if (dweight) *dweight = like(weight);
+    if (dbias) *dbias = like(bias);
+    run(ctamd_group_norm_backward_f32(x.fptr(), weight.fptr(), bias.fptr(), stats.fptr(), int(act), g.fptr(), dx ? dx->fptr() : nullptr,
+                                      dweight ? dweight->fptr() : nullptr, dbias ? dbias->fptr() : nullptr, n, p, c, groups, current_stream()),
+        "group_norm gradient");
 }
 Tensor sum_all(const Tensor& a) {
     check_device(a, "sum");
@@ -435,6 +481,48 @@ void sgd_step_all(const std::vector<Tensor*>& params, const std::vector<Tensor>&
         n.push_back(params[i]->numel());
     }
     run(ctamd_sgd_step_multi_f32(p.data(), g.data(), n.data(), int(p.size()), lr, current_stream()), "sgd_step_all");
+}
+void muon_step_all(const std::vector<Tensor*>& params, const std::vector<Tensor>& grads, const std::vector<Tensor*>& momenta, float lr, float momentum,
+                   bool nesterov, float weight_decay, int steps) {
+    if (params.size() != grads.size() || params.size() != momenta.size())
+        Ctorch_Error::throwException(kP, ErrorType::DIMENSION, "muon_step_all: one gradient and one momentum per parameter");
+    std::vector<ctamd_muon_matrix> table;
+    for (size_t i = 0; i < params.size(); ++i) {
+        if (grads[i].is_cleared()) continue;
+        Tensor& p = *params[i];
+        Tensor& m = *momenta[i];
+        const Tensor& g = grads[i];
+        check_device(p, "muon_step_all");
+        check_device(m, "muon_step_all");
+        check_device(g, "muon_step_all");
+        if (p.dim() != 2 || g.sizes() != p.sizes() || m.sizes() != p.sizes() || !p.is_contiguous() || !g.is_contiguous() || !m.is_contiguous())
+            Ctorch_Error::throwException(kP, ErrorType::DIMENSION, "muon_step_all: contiguous matrices with gradients and momenta of their shape");
+        p.require_writable("muon_step_all");
+        m.require_writable("muon_step_all");
+        p.forget_known_value();                              // written in place
+        m.forget_known_value();
+        const size_t rows = p.sizes()[0], cols = p.sizes()[1];
+        table.push_back({p.fptr(), g.fptr(), m.fptr(), p.fptr(), m.fptr(), int64_t(rows), int64_t(cols),
+                         0.2f * std::sqrt(float(rows > cols ? rows : cols))});
+    }
+    size_t bytes = 0;
+    run(ctamd_muon_workspace(table.data(), int(table.size()), &bytes), "muon_step_all");
+    // from the pool, back to it at once: its next user's launches follow these on the same stream
+    Tensor work(ShapeTag{}, {(bytes + 3) / 4}, DType::kFloat, DeviceType::kAMD, false);
+    const ctamd_muon_options options{lr, momentum, weight_decay, 1e-7f, nesterov ? 1 : 0, steps, {3.4445f, -4.7750f, 2.0315f}};
+    run(ctamd_muon_step_f32(table.data(), int(table.size()), &options, work.raw_ptr(), bytes, current_stream()), "muon_step_all");
+}
+Tensor newton_schulz(const Tensor& g, int steps) {
+    check_device(g, "newton_schulz");
+    if ((g.dim() != 2 && g.dim() != 3) || !g.is_contiguous())
+        Ctorch_Error::throwException(kP, ErrorType::DIMENSION, "newton_schulz: a contiguous matrix, or a batch of them");
+    const int64_t batch = g.dim() == 3 ? int64_t(g.sizes()[0]) : 1, rows = int64_t(g.sizes()[g.dim() - 2]), cols = int64_t(g.sizes()[g.dim() - 1]);
+    size_t bytes = 0;
+    run(ctamd_newton_schulz_workspace(rows, cols, batch, &bytes), "newton_schulz");
+    Tensor work(ShapeTag{}, {(bytes + 3) / 4}, DType::kFloat, DeviceType::kAMD, false);
+    Tensor r = like(g);
+    run(ctamd_newton_schulz_f32(g.fptr(), r.fptr(), rows, cols, batch, steps, nullptr, 1e-7f, work.raw_ptr(), bytes, current_stream()), "newton_schulz");
+    return r;
 }
 size_t count_correct(const Tensor& pred, const Tensor& labels) {
     check_device(pred, "count_correct");

@@ -456,6 +456,62 @@ long cth_grad_reduce(int kind, const float* x, const long* xd, int xn, const int
         return -1;
     }
 }
+// y = x.group_norm(groups, w, b, act); with an upstream up (may be null) the gradients of sum(y * up)
+long cth_group_norm(const float* x, const long* xd, int xn, long groups, const float* w, const float* b, int act, float eps, float* y, const float* up,
+                    float* dx, float* dw, float* db) {
+    try {
+        AutoDiff ctx;
+        configure(ctx);
+        AutoDiffContext::Guard guard(&ctx);
+        Tensor tx = make(x, xd, xn), tw = make(w, xd + xn - 1, 1), tb = make(b, xd + xn - 1, 1);
+        for (Tensor* t : {&tx, &tw, &tb}) t->requires_grad(true);
+        Tensor r = tx.group_norm(size_t(groups), tw, tb, Activation(act), eps);
+        if (up) {
+            Tensor z = r * make(up, xd, xn);
+            Tensor s = z.sum();
+            backward(s);
+            emit(grad(tx), dx);
+            emit(grad(tw), dw);
+            emit(grad(tb), db);
+        }
+        return emit(r, y);
+    } catch (const std::exception&) {
+        return -1;
+    }
+}
+// one in-place step of ctorch_amd_host::muon_step_all on `count` matrices; wrong != 0: a momentum of another shape
+long cth_muon_step(int count, const long* dims, float** params, const float** grads, float** momenta, float lr, float decay, int nesterov, int steps,
+                   int wrong) {
+    try {
+        std::vector<Tensor> p, g, m;
+        for (int i = 0; i < count; ++i) {
+            p.push_back(make(params[i], dims + 2 * i, 2));
+            g.push_back(make(grads[i], dims + 2 * i, 2));
+            m.push_back(make(momenta[i], dims + 2 * i, 2));
+        }
+        if (wrong) m[0] = Tensor::view_rows(m[0], 0, 1);
+        std::vector<Tensor*> pp, mm;
+        for (int i = 0; i < count; ++i) {
+            pp.push_back(&p[i]);
+            mm.push_back(&m[i]);
+        }
+        ctorch_amd_host::muon_step_all(pp, g, mm, lr, 0.95f, nesterov != 0, decay, steps);
+        for (int i = 0; i < count; ++i) {
+            emit(p[i], params[i]);
+            emit(m[i], momenta[i]);
+        }
+        return count;
+    } catch (const std::exception&) {
+        return -1;
+    }
+}
+long cth_newton_schulz(const float* g, const long* gd, int gn, int steps, float* out) {
+    try {
+        return emit(ctorch_amd_host::newton_schulz(make(g, gd, gn), steps), out);
+    } catch (const std::exception&) {
+        return -1;
+    }
+}
 long cth_log_softmax(const float* a, const long* ad, int an, int dim, float* out) {
     try {
         return emit(make(a, ad, an).log_softmax(dim), out);
@@ -1336,7 +1392,9 @@ float cth_mnist_accuracy(const float* pred, const float* labels, long rows) {
 // sums and a tape cleared after every step; 2: as 0 with the step recorded into a DeviceGraph at
 // the first batch and replayed for every batch (with unrelated eager work between the replays).
 // Adding 4 to the mode makes each layer one fused operator and the optimiser update one launch
-// (same values); adding 8 as well, the last layer and its loss are the one-pass head.  Parameters are written back; losses_out[s] = loss of step s.  ms_out (may be null) = milliseconds for all the steps.
+// (same values); adding 8 as well, the last layer and its loss are the one-pass head; adding 32, the
+// hidden layers are normalised over 8 groups; adding 64, the weight matrices are updated by their
+// orthogonalised momentum with a rate of 0.02.  Parameters are written back; losses_out[s] = loss of step s.  ms_out (may be null) = milliseconds for all the steps.
 long cth_mnist_train(const float* images, const float* labels, long n_images, long I, long H1, long H2, long C,
                      float* W1, float* b1, float* W2, float* b2, float* W3, float* b3, long batch, long steps,
                      float lr, int mode_bits, float* losses_out, double* ms_out) {
@@ -1348,6 +1406,8 @@ long cth_mnist_train(const float* images, const float* labels, long n_images, lo
         NeuralNetwork model(W1, b1, W2, b2, W3, b3, size_t(I), size_t(H1), size_t(H2), size_t(C), lr);
         model.fused_layers = fused;
         model.fused_head = (mode_bits & 8) != 0;
+        if (mode_bits & 32) model.normalise(8);
+        if (mode_bits & 64) model.use_muon(0.02f);
         const long num_batches = n_images / batch;
         AutoDiff autodiff;
         if (reference_tape == 1) {
@@ -1426,6 +1486,8 @@ long cth_mnist_demo(const char* dir, int epochs, int batch, float lr, int hidden
         opt.fused_layers = (mode_bits & 4) != 0;
         opt.fused_head = (mode_bits & 8) != 0;
         opt.loss_on_device = (mode_bits & 16) == 0;       // 16: every step reads its loss
+        opt.norm_groups = (mode_bits & 32) ? 8 : 0;
+        opt.muon_rate = (mode_bits & 64) ? 0.02f : 0.0f;
         opt.reference_tape = reference_tape == 1;
         opt.use_graph = reference_tape == 2;          // 2: live leaves and the step replayed from a recorded graph
         MnistDemoResult r = run_mnist_demo(opt);
