@@ -377,11 +377,11 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
     // What the epilogue adds to the sums.  A wave of few tiles asks for it now: at the end it would wait for it.
     auto mine = [&](int tile) { return C::KG == 1 || unsigned(tile) % C::KG == group; };
     const char* addend = KIND == POLY ? buf_a(j, work) : buf_y(j, work, from);
-    auto addend_at = [&](int a, int b, int quad) {
-        return pair_at(rows_q, j0 + wn + b * 32 + (lane & 31), i0 + wm + a * 32 + quad * 8) + (lane >> 5) * 8;
+    auto addend_at = [&](int a, int b, int side) {
+        return reinterpret_cast<const h8*>(addend + pair_at(rows_q, j0 + wn + b * 32 + (lane & 31), i0 + wm + a * 32 + side * 16 + (lane >> 5) * 8));
     };
-    constexpr bool kEarly = KIND != GRAM && C::TM * C::TN <= 4;
-    h4 old_hi[kEarly ? C::TM : 1][kEarly ? C::TN : 1][4], old_lo[kEarly ? C::TM : 1][kEarly ? C::TN : 1][4];
+    constexpr bool kEarly = KIND != GRAM && C::TM * C::TN * C::THREADS <= 2048;      // where the registers allow it
+    h8 early[kEarly ? C::TM : 1][kEarly ? C::TN : 1][2][2];
     if (kEarly) {
 #pragma unroll
         for (int a = 0; a < C::TM; ++a)
@@ -389,9 +389,9 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
             for (int b = 0; b < C::TN; ++b) {
                 if (!mine(a * C::TN + b) || i0 + wm + a * 32 >= rows_p || j0 + wn + b * 32 >= rows_q) continue;
 #pragma unroll
-                for (int quad = 0; quad < 4; ++quad) {
-                    old_hi[kEarly ? a : 0][kEarly ? b : 0][quad] = *reinterpret_cast<const h4*>(addend + addend_at(a, b, quad));
-                    old_lo[kEarly ? a : 0][kEarly ? b : 0][quad] = *reinterpret_cast<const h4*>(addend + addend_at(a, b, quad) + 16);
+                for (int side = 0; side < 2; ++side) {
+                    early[kEarly ? a : 0][kEarly ? b : 0][side][0] = addend_at(a, b, side)[0];
+                    early[kEarly ? a : 0][kEarly ? b : 0][side][1] = addend_at(a, b, side)[1];
                 }
             }
     }
@@ -506,6 +506,8 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
     char* turned = KIND == GRAM ? buf_a(j, work) : KIND == POLY ? buf_b(j, work) : buf_y(j, work, from ^ 1);
     uint32_t* s_turn = reinterpret_cast<uint32_t*>(piece(wave));       // a 32 x 32 tile per wave is turned in LDS
     const unsigned half = lane >> 5, col = lane & 31;
+    // four words of a row, placed so that rows r and r + 8, and one column of 16 rows, lie in all 64 banks
+    auto turn_at = [](unsigned row, unsigned four) { return (row ^ (row >> 3 & 1)) * 32 + ((four ^ (row >> 1)) & 7) * 4; };
 #pragma unroll
     for (int a = 0; a < C::TM; ++a)
 #pragma unroll
@@ -513,27 +515,33 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
             const unsigned gi = i0 + wm + a * 32, gj = j0 + wn + b * 32;
             if (!mine(a * C::TN + b) || gi >= rows_p || gj >= rows_q) continue;     // wave-uniform; rows are multiples of 64
 #pragma unroll
-            for (int quad = 0; quad < 4; ++quad) {
-                const size_t at = pair_at(rows_q, gj + col, gi + quad * 8) + half * 8;
-                float v[4];
+            for (int side = 0; side < 2; ++side) {
+                // rows 16 side + 8 half + 0 .. 7 of the tile in this lane, after the halves have exchanged four
+                float v[8];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[a][b][quad * 4 + e];
+                for (int e = 0; e < 4; ++e) {
+                    const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[a][b][side * 8 + e]),
+                                                                    __float_as_uint(acc[a][b][side * 8 + 4 + e]), false, false);
+                    v[e] = __uint_as_float(w[0]);
+                    v[4 + e] = __uint_as_float(w[1]);
+                }
+                const unsigned x0 = gi + side * 16 + half * 8;
                 if (KIND == GRAM) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] *= kScaleA / (kScaleX * kScaleX);
+                    for (int e = 0; e < 8; ++e) v[e] *= kScaleA / (kScaleX * kScaleX);
                 } else {
-                    const h4 oh = kEarly ? old_hi[kEarly ? a : 0][kEarly ? b : 0][quad] : *reinterpret_cast<const h4*>(addend + addend_at(a, b, quad));
-                    const h4 ol = kEarly ? old_lo[kEarly ? a : 0][kEarly ? b : 0][quad] : *reinterpret_cast<const h4*>(addend + addend_at(a, b, quad) + 16);
+                    const h8 oh = kEarly ? early[kEarly ? a : 0][kEarly ? b : 0][side][0] : addend_at(a, b, side)[0];
+                    const h8 ol = kEarly ? early[kEarly ? a : 0][kEarly ? b : 0][side][1] : addend_at(a, b, side)[1];
                     const float f = KIND == POLY ? cc / kScaleA : KIND == STEP ? 1.0f / kScaleA : 1.0f / (kScaleA * kScaleX);
                     const float old = KIND == POLY ? cb : KIND == STEP ? ca : ca / kScaleX;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = v[e] * f + old * (float(oh[e]) + float(ol[e]));
+                    for (int e = 0; e < 8; ++e) v[e] = v[e] * f + old * (float(oh[e]) + float(ol[e]));
                 }
                 if (KIND == LAST) {
-                    const unsigned x0 = gi + quad * 8 + half * 4, y = gj + col;
+                    const unsigned y = gj + col;
                     if (y < unsigned(j.n)) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
+                        for (int e = 0; e < 8; ++e)
                             if (x0 + e < unsigned(j.m)) {
                                 const size_t o = item * j.stride + (j.tall ? size_t(y) * j.cols + x0 + e : size_t(x0 + e) * j.cols + y);
                                 j.out[o] = result_at(t, j, o, v[e]);
@@ -541,19 +549,18 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
                     }
                     continue;
                 }
-                h4 hi, lo;
+                h8 hi, lo;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+                for (int e = 0; e < 8; ++e) {
                     hi[e] = _Float16(v[e]);
                     lo[e] = _Float16(v[e] - float(hi[e]));
-                    const unsigned row = quad * 8 + half * 4 + e;
-                    const uint32_t word = uint32_t(__builtin_bit_cast(uint16_t, _Float16(hi[e]))) |
-                                          (uint32_t(__builtin_bit_cast(uint16_t, _Float16(lo[e]))) << 16);
-                    s_turn[row * 32 + ((((col >> 2) ^ row) & 7) << 2) + (col & 3)] = word;
+                    s_turn[turn_at(side * 16 + half * 8 + e, col >> 2) + (col & 3)] =
+                        uint32_t(__builtin_bit_cast(uint16_t, _Float16(hi[e]))) | (uint32_t(__builtin_bit_cast(uint16_t, _Float16(lo[e]))) << 16);
                 }
                 if (mirror) {
-                    *reinterpret_cast<h4*>(turned + at) = hi;
-                    *reinterpret_cast<h4*>(turned + at + 16) = lo;
+                    h8* dst = reinterpret_cast<h8*>(turned + pair_at(rows_q, gj + col, x0));
+                    dst[0] = hi;
+                    dst[1] = lo;
                 }
             }
             if (KIND == LAST) continue;
@@ -561,9 +568,9 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const unsigned row = lane >> 1, c8 = 2 * h + (lane & 1);
-                const u4 w0 = *reinterpret_cast<const u4*>(s_turn + row * 32 + (((2 * c8) ^ row) & 7) * 4);
-                const u4 w1 = *reinterpret_cast<const u4*>(s_turn + row * 32 + (((2 * c8 + 1) ^ row) & 7) * 4);
+                const unsigned row = lane & 31, c8 = 2 * h + half;
+                const u4 w0 = *reinterpret_cast<const u4*>(s_turn + turn_at(row, 2 * c8));
+                const u4 w1 = *reinterpret_cast<const u4*>(s_turn + turn_at(row, 2 * c8 + 1));
                 u4 hi, lo;
                 hi[0] = (w0[0] & 0xffffu) | (w0[1] << 16);
                 hi[1] = (w0[2] & 0xffffu) | (w0[3] << 16);
@@ -1058,6 +1065,7 @@ void shape_job(Job* j, int64_t rows, int64_t cols, unsigned count) {
 
 typedef TileCfg<32, 32, 32, 4, 4, 4> Tile32;
 typedef TileCfg<64, 32, 32, 4, 4, 4> Tile64;
+typedef TileCfg<96, 96, 32, 4, 4, 3> Tile96;
 typedef TileCfg<128, 64, 64, 2, 2, 4> Tile128;
 typedef TileCfg<192, 96, 96, 2, 2, 3> Tile192;
 typedef TileCfg<256, 128, 64, 1, 1, 4> Tile256;
@@ -1085,7 +1093,8 @@ unsigned full_tiles(const Job& j, unsigned bt) { return ((unsigned(j.mp) + bt - 
 // block takes per k, measured (us per 1024 k, launch taken off, one block on every CU): a small tile waits
 // for its loads, a large one for the matrix cores - 4 times the work in 2.3 times the time from 64 to 128.
 //   4096 x 4096, X X^T: 253 tiles of 192 in 205 us, 136 of 256 in 265, 528 of 128 in 258;  B X: 256 tiles of
-//   256 in 350 us, 484 of 192 in 417;  2048 x 2048: 136 of 128 in 48 us, 528 of 64 in 57, 66 of 192 in 81;
+//   256 in 350 us, 484 of 192 in 417;  2048 x 2048: 253 of 96 in 40 us, 136 of 128 in 48, 528 of 64 in 57,
+//   66 of 192 in 81;  1500 x 1500, B X: 256 of 96 in 31 us, 144 of 128 in 37, 576 of 64 in 50;
 //   1024 x 1024: 136 of 64 in 12 us, 36 of 128 in 23;  333 x 1000: 78 of 32 in 8.6 us, 21 of 64 in 11.4.
 template <class F>
 int pick_tile(const Table& t, F tiles) {
@@ -1094,7 +1103,7 @@ int pick_tile(const Table& t, F tiles) {
         int tile, resident;                           // blocks per CU (by LDS)
         double cost;
     };
-    const Choice choices[5] = {{256, 1, 64.0}, {192, 1, 38.0}, {128, 1, 18.0}, {64, 1, 8.0}, {32, 2, 5.5}};
+    const Choice choices[6] = {{256, 1, 64.0}, {192, 1, 38.0}, {128, 1, 18.0}, {96, 1, 14.0}, {64, 1, 8.0}, {32, 2, 5.5}};
     int best = 0;
     double least = 1e300;
     for (const Choice& c : choices) {
@@ -1120,6 +1129,7 @@ void launch_product(int tile, Table* t, int from, const float* c, hipStream_t s)
     if (tile == 256) launch_product<Tile256, KIND>(t, from, c, s);
     else if (tile == 192) launch_product<Tile192, KIND>(t, from, c, s);
     else if (tile == 128) launch_product<Tile128, KIND>(t, from, c, s);
+    else if (tile == 96) launch_product<Tile96, KIND>(t, from, c, s);
     else if (tile == 64) launch_product<Tile64, KIND>(t, from, c, s);
     else launch_product<Tile32, KIND>(t, from, c, s);
 }
