@@ -19,6 +19,7 @@
 // its number, so that the 16 lanes that the 64 banks serve at once (of a ds_read_b128 per 32 x 16 operand
 // half) meet no bank twice.  Both operands of every product are read along their rows (A and B are symmetric;
 // X is kept with its transpose Y), so one kernel serves all three.
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -217,8 +218,12 @@ __global__ __launch_bounds__(kThreads) void load_pairs(Table t) {
     }
 }
 
+// The result of element i, whose parameter is `was`
+__device__ __forceinline__ float result_of(const Table& t, const Job& j, float was, float o) {
+    return j.param ? was * t.decay - j.step * o : o;
+}
 __device__ __forceinline__ float result_at(const Table& t, const Job& j, size_t i, float o) {
-    return j.param ? j.param[i] * t.decay - j.step * o : o;
+    return result_of(t, j, j.param ? j.param[i] : 0.0f, o);
 }
 
 // steps == 0: the normalised update is the result
@@ -381,7 +386,27 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
         return reinterpret_cast<const h8*>(addend + pair_at(rows_q, j0 + wn + b * 32 + (lane & 31), i0 + wm + a * 32 + side * 16 + (lane >> 5) * 8));
     };
     constexpr bool kEarly = KIND != GRAM && C::TM * C::TN * C::THREADS <= 2048;      // where the registers allow it
-    h8 early[kEarly ? C::TM : 1][kEarly ? C::TN : 1][2][2];
+    constexpr int kSlots = (C::TM * C::TN + C::KG - 1) / C::KG;                    // tiles that are the wave's own in the end
+    h8 early[kEarly ? kSlots : 1][2][2];
+    auto slot = [](int tile) { return kEarly ? tile / C::KG : 0; };
+    // and what the result is subtracted from: LAST with a parameter
+    const size_t step_x = j.tall ? 1 : size_t(j.cols), step_y = j.tall ? size_t(j.cols) : 1;
+    const size_t first = item * j.stride + (i0 + wm) * step_x + (j0 + wn) * step_y;                // of the wave, uniform
+    const size_t of_lane = (lane >> 5) * 8 * step_x + (lane & 31) * step_y;
+    auto element = [&](int a, int b, int side, int e) { return first + (a * 32 + side * 16 + e) * step_x + b * 32 * step_y; };
+    auto inside = [&](int a, int b, int side, int e) {
+        return j0 + wn + b * 32 + (lane & 31) < unsigned(j.n) && i0 + wm + a * 32 + side * 16 + (lane >> 5) * 8 + e < unsigned(j.m);
+    };
+    constexpr bool kParam = kEarly && KIND == LAST;
+    float was[kParam ? kSlots : 2][2][8];            // late: of a tile and of the wave's next
+    auto ask = [&](int tile, int into) {
+        const int a = tile / C::TN, b = tile % C::TN;
+#pragma unroll
+        for (int side = 0; side < 2; ++side)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (inside(a, b, side, e)) was[into][side][e] = (j.param + of_lane)[element(a, b, side, e)];
+    };
     if (kEarly) {
 #pragma unroll
         for (int a = 0; a < C::TM; ++a)
@@ -390,9 +415,10 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
                 if (!mine(a * C::TN + b) || i0 + wm + a * 32 >= rows_p || j0 + wn + b * 32 >= rows_q) continue;
 #pragma unroll
                 for (int side = 0; side < 2; ++side) {
-                    early[kEarly ? a : 0][kEarly ? b : 0][side][0] = addend_at(a, b, side)[0];
-                    early[kEarly ? a : 0][kEarly ? b : 0][side][1] = addend_at(a, b, side)[1];
+                    early[slot(a * C::TN + b)][side][0] = addend_at(a, b, side)[0];
+                    early[slot(a * C::TN + b)][side][1] = addend_at(a, b, side)[1];
                 }
+                if (kParam && j.param) ask(a * C::TN + b, kParam ? slot(a * C::TN + b) : 0);
             }
     }
     load(s_ring0, 0);
@@ -513,6 +539,11 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
 #pragma unroll
         for (int b = 0; b < C::TN; ++b) {
             const unsigned gi = i0 + wm + a * 32, gj = j0 + wn + b * 32;
+            if (KIND == LAST && !kParam && j.param && mine(a * C::TN + b)) {
+                // a tile ahead, and before this one's stores: a result may lie where its parameter was
+                if (a * C::TN + b < C::KG) ask(a * C::TN + b, 0);
+                if (a * C::TN + b + C::KG < C::TM * C::TN) ask(a * C::TN + b + C::KG, ((a * C::TN + b) / C::KG + 1) & 1);
+            }
             if (!mine(a * C::TN + b) || gi >= rows_p || gj >= rows_q) continue;     // wave-uniform; rows are multiples of 64
 #pragma unroll
             for (int side = 0; side < 2; ++side) {
@@ -530,23 +561,18 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] *= kScaleA / (kScaleX * kScaleX);
                 } else {
-                    const h8 oh = kEarly ? early[kEarly ? a : 0][kEarly ? b : 0][side][0] : addend_at(a, b, side)[0];
-                    const h8 ol = kEarly ? early[kEarly ? a : 0][kEarly ? b : 0][side][1] : addend_at(a, b, side)[1];
+                    const h8 oh = kEarly ? early[slot(a * C::TN + b)][side][0] : addend_at(a, b, side)[0];
+                    const h8 ol = kEarly ? early[slot(a * C::TN + b)][side][1] : addend_at(a, b, side)[1];
                     const float f = KIND == POLY ? cc / kScaleA : KIND == STEP ? 1.0f / kScaleA : 1.0f / (kScaleA * kScaleX);
                     const float old = KIND == POLY ? cb : KIND == STEP ? ca : ca / kScaleX;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] = v[e] * f + old * (float(oh[e]) + float(ol[e]));
                 }
                 if (KIND == LAST) {
-                    const unsigned y = gj + col;
-                    if (y < unsigned(j.n)) {
+                    const float (&old_param)[8] = was[kParam ? slot(a * C::TN + b) : (a * C::TN + b) / C::KG & 1][side];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (x0 + e < unsigned(j.m)) {
-                                const size_t o = item * j.stride + (j.tall ? size_t(y) * j.cols + x0 + e : size_t(x0 + e) * j.cols + y);
-                                j.out[o] = result_at(t, j, o, v[e]);
-                            }
-                    }
+                    for (int e = 0; e < 8; ++e)
+                        if (inside(a, b, side, e)) (j.out + of_lane)[element(a, b, side, e)] = result_of(t, j, old_param[e], v[e]);
                     continue;
                 }
                 h8 hi, lo;
@@ -1089,28 +1115,61 @@ unsigned sym_tiles(const Job& j, unsigned bt) {
 }
 unsigned full_tiles(const Job& j, unsigned bt) { return ((unsigned(j.mp) + bt - 1) / bt) * ((unsigned(j.np) + bt - 1) / bt); }
 
-// The tile of a launch: the one whose rounds over the chip cost least.  The cost of a round is the time a
-// block takes per k, measured (us per 1024 k, launch taken off, one block on every CU): a small tile waits
-// for its loads, a large one for the matrix cores - 4 times the work in 2.3 times the time from 64 to 128.
-//   4096 x 4096, X X^T: 253 tiles of 192 in 205 us, 136 of 256 in 265, 528 of 128 in 258;  B X: 256 tiles of
-//   256 in 350 us, 484 of 192 in 417;  2048 x 2048: 253 of 96 in 40 us, 136 of 128 in 48, 528 of 64 in 57,
-//   66 of 192 in 81;  1500 x 1500, B X: 256 of 96 in 31 us, 144 of 128 in 37, 576 of 64 in 50;
-//   1024 x 1024: 136 of 64 in 12 us, 36 of 128 in 23;  333 x 1000: 78 of 32 in 8.6 us, 21 of 64 in 11.4.
-template <class F>
-int pick_tile(const Table& t, F tiles) {
+// The tile of a launch: the one with which its blocks, longest first, are estimated to be done soonest.  A
+// block takes `fixed` us and `per_k` us per 1024 k while most of the chip is idle; with all CUs at work the
+// clock gives way to the power limit and memory is shared, and everything takes `busy` times as long.  All three
+// were measured, at 2 to 1849 blocks and k from 512 to 4096.  In us, the nearest others beside the choice:
+//   4096 x 4096, X X^T: 253 tiles of 192 in 205, 136 of 256 in 252, 528 of 128 in 253;  B X: 256 of 256 in
+//   345, 484 of 192 in 404, 1024 of 128 in 403;  2048 x 2048, X X^T: 253 of 96 in 41, 136 of 128 in 47,
+//   66 of 192 in 78;  B X: 256 of 128 in 61, 484 of 96 in 78, 64 of 256 in 125;  1024 x 1024, X X^T: 136 of 64
+//   in 11.5, 66 of 96 in 16.6;  512 x 512, X X^T: 136 of 32 in 6.7, 36 of 64 in 8.3.
+// A parameter's update takes a block `param` us more: a large tile's wave has no registers to ask for all of
+// its part before it has its sums (784 x 2048, 2048 x 2048, 2048 x 4096 and 4096 x 1001 together: tiles of 256
+// in 198 us without and 281 with it, of 128 in 220 and 251).
+template <class F, class K>
+int pick_tile(const Table& t, F tiles, K k, bool params = false) {
     const size_t cus = size_t(compute_units() > 0 ? compute_units() : 256);
     struct Choice {
         int tile, resident;                           // blocks per CU (by LDS)
-        double cost;
+        double fixed, per_k, busy, param;
     };
-    const Choice choices[6] = {{256, 1, 64.0}, {192, 1, 38.0}, {128, 1, 18.0}, {96, 1, 14.0}, {64, 1, 8.0}, {32, 2, 5.5}};
+    const Choice choices[6] = {{256, 1, 21.0, 48.0, 1.6, 50.0}, {192, 1, 18.0, 31.0, 1.5, 30.0}, {128, 1, 12.0, 14.0, 1.5, 10.0},
+                               {96, 1, 6.0, 10.6, 1.3, 10.0},   {64, 1, 5.5, 4.6, 1.3, 4.0},     {32, 2, 5.2, 2.9, 1.3, 2.0}};
     int best = 0;
     double least = 1e300;
     for (const Choice& c : choices) {
-        size_t blocks = 0;
-        for (int j = 0; j < t.jobs; ++j) blocks += size_t(t.job[j].count) * tiles(t.job[j], unsigned(c.tile));
-        const size_t at_once = cus * size_t(c.resident);
-        const double cost = double((blocks + at_once - 1) / at_once) * c.cost;
+        // the places for a block, by the time at which they fall free: a few levels, ascending
+        struct Level {
+            double free_at;
+            size_t places;
+        } level[2 * kMaxJobs + 2] = {{0.0, cus * size_t(c.resident)}};
+        int levels = 1;
+        const size_t places = level[0].places;
+        double sum = 0, done = 0;
+        for (int j = 0; j < t.jobs; ++j) {            // longest first: by_k() has sorted them
+            size_t blocks = size_t(t.job[j].count) * tiles(t.job[j], unsigned(c.tile));
+            const double each = c.fixed + c.per_k * double(k(t.job[j])) / 1024.0 + (params ? c.param : 0.0);
+            sum += double(blocks) * each;
+            const size_t rounds = blocks / places;
+            blocks %= places;
+            for (int l = 0; l < levels; ++l) level[l].free_at += double(rounds) * each;
+            while (blocks) {                          // fewer than the places: each is taken once at most
+                Level first = level[0];
+                const size_t taken = blocks < first.places ? blocks : first.places;
+                blocks -= taken;
+                level[0].places -= taken;
+                if (!level[0].places) {
+                    --levels;
+                    for (int l = 0; l < levels; ++l) level[l] = level[l + 1];
+                }
+                int at = levels++;
+                for (; at > 0 && level[at - 1].free_at > first.free_at + each; --at) level[at] = level[at - 1];
+                level[at] = {first.free_at + each, taken};
+            }
+        }
+        for (int l = 0; l < levels; ++l)
+            if (level[l].free_at > done) done = level[l].free_at;
+        const double cost = done * (1.0 + (c.busy - 1.0) * sum / (done * double(places)));
         if (cost < least) {
             least = cost;
             best = c.tile;
@@ -1118,6 +1177,15 @@ int pick_tile(const Table& t, F tiles) {
     }
     return best;
 }
+
+// Sorts the matrices by the length of a launch's sums, longest first: blocks are given out in order, and short
+// ones fill what long ones leave.
+template <class K>
+void by_k(Table* t, K k) {
+    std::stable_sort(t->job, t->job + t->jobs, [&](const Job& a, const Job& b) { return k(a) > k(b); });
+}
+int gram_k(const Job& j) { return j.np; }
+int square_k(const Job& j) { return j.mp; }
 
 template <class C, Kind KIND>
 void launch_product(Table* t, int from, const float* c, hipStream_t s) {
@@ -1135,13 +1203,19 @@ void launch_product(int tile, Table* t, int from, const float* c, hipStream_t s)
 }
 
 int iterate(const char* who, Table* t, int steps, const float* c, hipStream_t s) {
-    const int sym = pick_tile(*t, sym_tiles), full = pick_tile(*t, full_tiles);
+    by_k(t, square_k);
+    const int poly = pick_tile(*t, sym_tiles, square_k), full = pick_tile(*t, full_tiles, square_k);
+    const int last = pick_tile(*t, full_tiles, square_k, t->job[0].param != nullptr);
+    by_k(t, gram_k);
+    const int gram = pick_tile(*t, sym_tiles, gram_k);
     for (int k = 0; k < steps; ++k) {
         const int from = k & 1;
-        launch_product<GRAM>(sym, t, from, c, s);
-        launch_product<POLY>(sym, t, from, c, s);
+        by_k(t, gram_k);
+        launch_product<GRAM>(gram, t, from, c, s);
+        by_k(t, square_k);
+        launch_product<POLY>(poly, t, from, c, s);
         if (k + 1 < steps) launch_product<STEP>(full, t, from, c, s);
-        else launch_product<LAST>(full, t, from, c, s);
+        else launch_product<LAST>(last, t, from, c, s);
         const int rc = launched(who);
         if (rc) return rc;
     }
