@@ -21,6 +21,8 @@
 // X is kept with its transpose Y), so one kernel serves all three.
 #include <algorithm>
 #include <cmath>
+#include <memory>
+#include <new>
 #include <type_traits>
 
 #include "common.h"
@@ -248,8 +250,13 @@ __global__ __launch_bounds__(kThreads) void scaled_update(Table t) {
 enum Kind { GRAM, POLY, STEP, LAST };
 
 // A block computes a BT x BT tile.  Its waves stand in (BT / WM) x (BT / WN) positions, KG waves to a
-// position, and those share the k range: a stage of the ring is a slab of 16 k for each group (a large wave tile reads each fragment from LDS for more MFMAs; on a small
-// block tile only the k range is left to share).  RING stages, all but one on their way.
+// position, and those share the k range: a stage of the ring is a slab of 16 k for each group (a large wave tile
+// reads each fragment from LDS for more MFMAs; on a small block tile only the k range is left to share).
+// RING stages, all but one on their way.  A launch costs 5 - 20 us beside its sums, for the first loads'
+// latency and the stores (2048 x 2048 with all but 4 of its 64 stages left out: 14 of 45 us).  Loads alone,
+// MFMAs alone and reads from LDS alone would each take 70 - 85 % of the time on the tiles of 128 and
+// less: what they miss is a perfect overlap, which neither fragments read a stage ahead nor MFMAs spread
+// between the loads brought nearer (47.0 against 46.9 us).
 template <int BT_, int WM_, int WN_, int KG_, int F_, int RING_>
 struct TileCfg {
     static constexpr int BT = BT_, WM = WM_, WN = WN_, KG = KG_, F = F_, RING = RING_;
@@ -1370,6 +1377,38 @@ static size_t next_table(const ctamd_muon_matrix* matrices, int count, int* at, 
     return bytes;
 }
 
+// Whether a tensor that the call writes shares memory with another of its tensors: the matrices of a table
+// run side by side, so that one given twice would get one step or a mixture of two.  -1: out of memory
+static int tensors_overlap(const ctamd_muon_matrix* matrices, int count) {
+    struct Extent {
+        uintptr_t from, to;
+        bool written;
+    };
+    std::unique_ptr<Extent[]> all(new (std::nothrow) Extent[size_t(count) * 5 + 1]);
+    if (!all) return -1;
+    size_t n = 0;
+    for (int i = 0; i < count; ++i) {
+        const ctamd_muon_matrix& a = matrices[i];
+        const size_t bytes = size_t(a.rows) * size_t(a.cols) * sizeof(float);
+        if (!bytes) continue;
+        auto add = [&](const float* p, bool written) { all[n++] = {reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes, written}; };
+        add(a.grad, false);
+        add(a.new_param, true);
+        add(a.new_momentum, true);
+        if (a.param != a.new_param) add(a.param, false);
+        if (a.momentum != a.new_momentum) add(a.momentum, false);
+    }
+    std::sort(all.get(), all.get() + n, [](const Extent& a, const Extent& b) { return a.from < b.from; });
+    uintptr_t any = 0, written = 0;                  // ends of what was met so far
+    for (size_t i = 0; i < n; ++i) {
+        const Extent& e = all[i];
+        if (e.from < (e.written ? any : written)) return 1;
+        if (e.to > any) any = e.to;
+        if (e.written && e.to > written) written = e.to;
+    }
+    return 0;
+}
+
 int ctamd_muon_workspace(const ctamd_muon_matrix* matrices, int count, size_t* bytes_host) {
     if (!bytes_host) return fail(CTAMD_EINVAL, "%s: null output", __func__);
     *bytes_host = 0;
@@ -1400,6 +1439,8 @@ int ctamd_muon_step_f32(const ctamd_muon_matrix* matrices, int count, const ctam
         if (a.rows && a.cols && (!a.param || !a.grad || !a.momentum || !a.new_param || !a.new_momentum))
             return fail(CTAMD_EINVAL, "%s: null tensor in matrix %d", __func__, i);
     }
+    const int overlap = tensors_overlap(matrices, count);
+    if (overlap) return fail(CTAMD_EINVAL, overlap < 0 ? "%s: out of host memory" : "%s: a tensor that is written overlaps another", __func__);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return fail(CTAMD_EINVAL, "%s: a workspace of %zu bytes, 16-byte aligned, is needed", __func__, need);
     Table t{};

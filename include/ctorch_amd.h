@@ -372,7 +372,8 @@ int ctamd_matmul_relu_mask_f32(const float* a, int64_t as0, int64_t as1, const f
  * (for rows > cols on the transposed matrix; the result is the same), `batch` matrices one after the other
  * in memory.  coefficients_host (HOST, may be NULL): a, b, c; NULL stands for 3.4445, -4.7750, 2.0315, which
  * in 5 steps take singular values of 0.005 |g|_F and more to 0.7 - 1.2.  Matrices are held as pairs of f16
- * numbers with 22 bits together and multiplied by the f16 matrix cores with fp32 sums: as close to the
+ * numbers with 22 bits together (three with 24 where no matrix of the call has more than 32 on its shorter
+ * side and 8192 on its longer) and multiplied by the f16 matrix cores with fp32 sums: as close to the
  * iteration in 64 bits as fp32 products are.  That holds while the entries of X stay below 8 and
  * those of A and b A + c A A below 32 (singular values below 4 or so; the given coefficients keep them below
  * 1.3); coefficients beyond 32 are CTAMD_EINVAL.  An update whose norm is far below eps comes out as zero
@@ -390,7 +391,8 @@ int ctamd_newton_schulz_f32(const float* g, float* out, int64_t rows, int64_t co
  *   U = options.nesterov ? grad + options.momentum * momentum' : momentum'
  *   new_param = param * (1 - learning_rate * weight_decay) - learning_rate * scale * orthogonalised(U)
  * with the iteration of ctamd_newton_schulz_f32 (options.steps, coefficients, eps).  new_param may be param
- * and new_momentum may be momentum (an update in place); no other two tensors may overlap.  scale is the
+ * and new_momentum may be momentum (an update in place); a tensor that is written and overlaps any other of the
+ * call's, a matrix given twice among them, is CTAMD_EINVAL.  scale is the
  * matrix's own factor, e.g. 0.2 * sqrt(max(rows, cols)) for updates as large as an adaptive optimiser's.
  * The matrices of a call share its launches (16 at a time).  Workspace as above, from
  * ctamd_muon_workspace.  Stands beside ctamd_sgd_step_multi_f32 for weight matrices; biases and other

@@ -193,6 +193,46 @@ def test_steps_against_64_bits(shapes, steps, nesterov):
         assert torch.equal(p, np_) and torch.equal(m, nm)
 
 
+@pytest.mark.parametrize("shapes", [[(1500, 1533)], [(2048, 2100), (4100, 1001), (784, 2048)], [(4096, 4160)], [(3500, 2050), (1000, 3490)]], ids=str)
+def test_large_steps(shapes):
+    """Every size of tile with a parameter to update, ragged at its edges; the 64-bit iteration by torch on the
+    device.  Bounds as tests/update_oracle.py's, of the Frobenius norm."""
+    import gpu_support as G
+    import torch
+    gen = torch.Generator(device=G.DEV)
+    gen.manual_seed(11)
+    lr, mu, decay, band = 0.02, 0.95, 0.01, 64
+    host = []
+    for rows, cols in shapes:
+        p, g, m = (torch.randn(rows, cols, device=G.DEV, generator=gen) * s for s in (1 / np.sqrt(rows), 1e-3, 5e-3))
+        guarded = [torch.full((rows * cols + 2 * band,), 7.5, device=G.DEV) for _ in range(2)]
+        out = [t[band:band + rows * cols].view(rows, cols) for t in guarded]
+        host.append((p, g, m, out, guarded, float(0.2 * np.sqrt(max(rows, cols)))))
+    _muon(G, [(p, g, m, *out, scale) for p, g, m, out, _, scale in host], _options(lr, mu, decay))
+    f = lambda v: float(np.float32(v))  # noqa: E731
+    a, b, c = (f(v) for v in O.COEFFICIENTS)
+    for p, g, m, (new, new_m), guarded, scale in host:
+        want_m = f(mu) * m.double() + g.double()
+        assert bool(((new_m.double() - want_m).abs() <= 2.0 ** -23 * ((f(mu) * m.double()).abs() + want_m.abs())).all())
+        x = g.double() + f(mu) * want_m
+        x = x / (x.norm() + f(1e-7))
+        tall = x.shape[0] > x.shape[1]
+        x = x.T.contiguous() if tall else x
+        for _ in range(5):
+            gram = x @ x.T.contiguous()
+            x = a * x + (b * gram + c * (gram @ gram)) @ x
+        o = x.T if tall else x
+        step = f(lr) * f(scale)
+        want = p.double() * (1 - f(lr) * f(decay)) - step * o
+        bound = step * (O.newton_schulz_bound(p.shape, 5) + a ** 5 * 2.0 ** -21) + 2.0 ** -22 * float((p.double().abs() + step * o.abs()).norm())
+        assert float((new.double() - want).norm()) <= bound, (tuple(p.shape), float((new.double() - want).norm()), bound)
+        assert all(bool((t[:band] == 7.5).all()) and bool((t[-band:] == 7.5).all()) for t in guarded)
+    # in place: the same bits
+    _muon(G, [(p, g, m, p, m, scale) for p, g, m, _, _, scale in host], _options(lr, mu, decay))
+    for p, _, m, (new, new_m), _, _ in host:
+        assert torch.equal(p, new) and torch.equal(m, new_m)
+
+
 def test_streams_replays_and_two_graphs():
     import gpu_support as G
     import torch

@@ -64,3 +64,28 @@ def test_refused_muon_calls():
     assert call(o=options(steps=65)) == -1 and call(o=options(eps=-1.0)) == -1 and call(o=options(coefficients=(40.0, 0.0, 0.0))) == -1
     assert lib.ctamd_muon_step_f32(table(), 1, None, None, 0, None) == -1
     assert call(count=0, work=None, nbytes=0) == 0 and call(table(rows=0, param=None), work=None, nbytes=0) == 0
+
+
+def test_a_written_tensor_may_not_overlap_another():
+    """The matrices of a call run side by side: a matrix given twice, or tensors that share memory, are refused."""
+    capi, lib = _lib()
+    opt = capi.MuonOptions(0.1, 0.9, 0.0, 1e-7, 1, 5, (C.c_float * 3)(3.0, -4.0, 2.0))
+    nbytes = 8 * 9 * 4
+    work = 1 << 20
+
+    def call(*mats):
+        table = (capi.MuonMatrix * len(mats))(*[capi.MuonMatrix(*m, 8, 9, 1.0) for m in mats])
+        size = C.c_size_t()
+        assert lib.ctamd_muon_workspace(table, len(mats), C.byref(size)) == 0
+        rc = lib.ctamd_muon_step_f32(table, len(mats), C.byref(opt), C.c_void_p(work), size.value, None)
+        return rc == -1 and b"overlaps" in lib.ctamd_last_error()
+    at = [4096 + 1024 * k for k in range(12)]
+    one = (at[0], at[1], at[2], at[0], at[2])
+    assert call(one, one)                                                             # twice the same
+    assert call(one, (at[3], at[4], at[5], at[0], at[6]))                             # two results in one place
+    assert call(one, (at[3], at[4], at[5], at[6], at[2]))
+    assert call(one, (at[3], at[0], at[5], at[6], at[7]))                             # another's gradient is written
+    assert call((at[0], at[1], at[2], at[1], at[3]))                                  # its own gradient
+    assert call((at[0], at[1], at[2], at[3], at[3]))
+    assert call((at[0], at[1], at[2], at[0] + 4, at[3]))                              # in place, but for one element
+    assert call((at[0], at[1], at[2], at[0] + nbytes - 4, at[3]))
