@@ -220,6 +220,8 @@ Tensor group_norm(const Tensor& x, size_t groups, const Tensor& weight, const Te
     channels_last(x, n, p, c, "group_norm");
     check_per_channel(weight, c, "group_norm");
     check_per_channel(bias, c, "group_norm");
+    if (groups == 0 || groups > c || c % groups != 0)        // before the statistics are allocated
+        Ctorch_Error::throwException(kP, ErrorType::DIMENSION, "group_norm: the channels do not divide into the groups");
     Tensor r = like(x);
     if (stats) *stats = Tensor(ShapeTag{}, {n, groups, 2}, DType::kFloat, DeviceType::kAMD, false);
     run(ctamd_group_norm_f32(x.fptr(), weight.fptr(), bias.fptr(), eps, int(act), r.fptr(), stats ? stats->fptr() : nullptr, n, p, c, groups,

@@ -74,6 +74,14 @@ def test_group_norm_refuses(host):
                                     None) == -1
 
 
+def test_more_groups_than_channels_are_refused_before_their_statistics_are_allocated(host):
+    print("case host group norm, 2^40 groups", flush=True)
+    x, w = np.ones((4, 6), np.float32), np.ones(6, np.float32)
+    assert _group_norm(host, x, 1 << 40, w, w, "none", up=x)[0] == -1
+    assert _group_norm(host, x, 12, w, w, "none")[0] == -1
+    assert _group_norm(host, x, 3, w, w, "none")[0] == x.size                  # and the next call is served
+
+
 def _grad(rows, cols, seed):
     r = np.random.default_rng(seed)
     return f32(1e-3 * r.standard_normal((rows, cols)))
