@@ -177,32 +177,37 @@ __global__ __launch_bounds__(kThreads) void load_pairs(Table t) {
     const unsigned tiles = (rp / 64) * (cp / 64), item = local / tiles, tile = local % tiles;
     const unsigned r0 = (tile / (cp / 64)) * 64, c0 = (tile % (cp / 64)) * 64;
     char* work = j.work + item * j.work_stride;
-    const double inv = inverse_norm(t, j, work, s_part);
     char* straight = j.tall ? buf_y(j, work, 0) : buf_x(j, work, 0);
     char* turned = j.tall ? buf_x(j, work, 0) : buf_y(j, work, 0);
+    float v[4][4];                                   // asked for before the norm's parts are waited for
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         const unsigned r = (threadIdx.x >> 4) + 16 * q, c = (threadIdx.x & 15) * 4;
         const size_t at = item * j.stride + size_t(r0 + r) * j.cols + c0 + c;
-        float v[4];
-        if (j.vec && int64_t(r0 + r) < j.rows && int64_t(c0 + c) < j.cols) {
-            v4f u = *reinterpret_cast<const v4f*>((j.momentum && !t.nesterov ? j.new_momentum : j.grad) + at);
-            if (j.momentum && t.nesterov) {
-                const v4f m = *reinterpret_cast<const v4f*>(j.new_momentum + at);
+        if (j.vec) {
+            v4f u = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (int64_t(r0 + r) < j.rows && int64_t(c0 + c) < j.cols) {
+                u = *reinterpret_cast<const v4f*>((j.momentum && !t.nesterov ? j.new_momentum : j.grad) + at);
+                if (j.momentum && t.nesterov) {
+                    const v4f m = *reinterpret_cast<const v4f*>(j.new_momentum + at);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) u[e] = u[e] + t.mu * m[e];
+                    for (int e = 0; e < 4; ++e) u[e] = u[e] + t.mu * m[e];
+                }
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = float(u[e] * inv);
+            for (int e = 0; e < 4; ++e) v[q][e] = u[e];
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const bool in = int64_t(r0 + r) < j.rows && int64_t(c0 + c + e) < j.cols;
-                v[e] = in ? float(update_at(t, j, at + e) * inv) : 0.0f;
-            }
+            for (int e = 0; e < 4; ++e) v[q][e] = int64_t(r0 + r) < j.rows && int64_t(c0 + c + e) < j.cols ? update_at(t, j, at + e) : 0.0f;
         }
+    }
+    const double inv = inverse_norm(t, j, work, s_part);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s_tile[r][c + e] = v[e];
+    for (int q = 0; q < 4; ++q) {
+        const unsigned r = (threadIdx.x >> 4) + 16 * q, c = (threadIdx.x & 15) * 4;
+        const bool row_in = int64_t(r0 + r) < j.rows;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s_tile[r][c + e] = row_in && int64_t(c0 + c + e) < j.cols ? float(v[q][e] * inv) : 0.0f;     // inf * 0 is no zero
     }
     __syncthreads();
     // 8 columns of a row to a thread: neighbouring threads fill neighbouring memory of a panel
@@ -1088,7 +1093,7 @@ void shape_job(Job* j, int64_t rows, int64_t cols, unsigned count) {
     j->count = count;
     j->stride = size_t(rows) * size_t(cols);
     size_t size = (j->stride + kNormParts - 1) / kNormParts;
-    size = (size + 4095) / 4096 * 4096;
+    size = (size + 1023) / 1024 * 1024;              // a vector for every thread
     j->part_size = size;
     j->norm_parts = unsigned((j->stride + size - 1) / size);
     j->work_stride = kNormBytes + 4 * pairs_xy(*j) + 2 * pairs_a(*j);
