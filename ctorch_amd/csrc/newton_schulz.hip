@@ -42,7 +42,7 @@ constexpr int kXcds = 8;
 constexpr float kScaleX = 8192.0f, kScaleA = 2048.0f;
 
 constexpr int kMaxJobs = 16;
-constexpr int kNormParts = 1024;
+constexpr int kNormParts = 1024, kCounters = 256;
 
 // One matrix - or `count` matrices of one shape, `stride` elements apart - of a call.
 struct Job {
@@ -61,6 +61,7 @@ struct Job {
     int vec;                     // every tensor and every row allows vectors of 4
     unsigned norm_parts;
     size_t part_size;            // elements per part of the norm
+    unsigned splits;             // parts of the sums of X X^T
 };
 struct Table {
     int jobs;
@@ -70,10 +71,11 @@ struct Table {
     int nesterov;
 };
 
-// workspace of one matrix: the norm's partial sums, X and Y twice, A, B
+// workspace of one matrix: the norm's partial sums, counters, X and Y twice, A, B
 __host__ __device__ inline size_t pairs_xy(const Job& j) { return size_t(j.mp) * j.np * 4; }
 __host__ __device__ inline size_t pairs_a(const Job& j) { return size_t(j.mp) * j.mp * 4; }
-constexpr size_t kNormBytes = kNormParts * sizeof(double);
+constexpr size_t kNormBytes = kNormParts * sizeof(double) + kCounters * sizeof(unsigned);
+__device__ inline unsigned* counters(char* w) { return reinterpret_cast<unsigned*>(w + kNormParts * sizeof(double)); }
 __device__ inline char* buf_x(const Job& j, char* w, int which) { return w + kNormBytes + size_t(which) * 2 * pairs_xy(j); }
 __device__ inline char* buf_y(const Job& j, char* w, int which) { return w + kNormBytes + (size_t(which) * 2 + 1) * pairs_xy(j); }
 __device__ inline char* buf_a(const Job& j, char* w) { return w + kNormBytes + 4 * pairs_xy(j); }
@@ -135,7 +137,10 @@ __global__ __launch_bounds__(kThreads) void momentum_norm(Table t) {
         sum += double(u) * double(u);
     }
     sum = block_sum(sum, s_part);
-    if (threadIdx.x == 0) reinterpret_cast<double*>(j.work + item * j.work_stride)[part] = sum;
+    char* work = j.work + item * j.work_stride;
+    if (threadIdx.x == 0) reinterpret_cast<double*>(work)[part] = sum;
+    if (part == 0)
+        for (unsigned i = threadIdx.x; i < kCounters; i += kThreads) counters(work)[i] = 0;
 }
 
 // 1 / (|U|_F + eps) from the parts; every thread gets it.  Kept in double: its product with an element of U
@@ -280,7 +285,60 @@ __device__ __forceinline__ void lds_load(const char* g, char* l) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)l, 16, 0, 0);
 }
 
-template <class C, Kind KIND>
+// A tile of 32 x 32 is stored as pairs twice, straight and transposed.  Its sums stand with a column to a lane:
+// the halves of a wave first exchange four rows, so that a lane has rows 16 side + 8 (lane / 32) + 0 .. 7 ...
+__device__ __forceinline__ void exchange(const v16f& acc, int side, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[side * 8 + e]), __float_as_uint(acc[side * 8 + 4 + e]), false, false);
+        v[e] = __uint_as_float(w[0]);
+        v[4 + e] = __uint_as_float(w[1]);
+    }
+}
+// ... which are 32 bytes of the transposed matrix ...
+__device__ __forceinline__ void pairs_of(const float (&v)[8], h8* hi, h8* lo) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        (*hi)[e] = _Float16(v[e]);
+        (*lo)[e] = _Float16(v[e] - float((*hi)[e]));
+    }
+}
+// ... and for the straight one the tile is turned in LDS, 4 KiB: four words of a row, placed so that rows r and
+// r + 8, and one column of 16 rows, lie in all 64 banks.
+__device__ __forceinline__ unsigned turn_at(unsigned row, unsigned four) { return (row ^ (row >> 3 & 1)) * 32 + ((four ^ (row >> 1)) & 7) * 4; }
+__device__ __forceinline__ void put_to_turn(uint32_t* s_turn, int side, unsigned lane, const h8& hi, const h8& lo) {
+    const unsigned half = lane >> 5, col = lane & 31;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        s_turn[turn_at(side * 16 + half * 8 + e, col >> 2) + (col & 3)] =
+            uint32_t(__builtin_bit_cast(uint16_t, _Float16(hi[e]))) | (uint32_t(__builtin_bit_cast(uint16_t, _Float16(lo[e]))) << 16);
+}
+// the tile's first row and column in the matrix of `rows` padded rows; a wave reads back only what it wrote itself
+__device__ __forceinline__ void store_turned(const uint32_t* s_turn, unsigned lane, char* to, unsigned rows, unsigned row0, unsigned col0) {
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const unsigned row = lane & 31, c8 = 2 * h + (lane >> 5);
+        const u4 w0 = *reinterpret_cast<const u4*>(s_turn + turn_at(row, 2 * c8));
+        const u4 w1 = *reinterpret_cast<const u4*>(s_turn + turn_at(row, 2 * c8 + 1));
+        u4 hi, lo;
+        hi[0] = (w0[0] & 0xffffu) | (w0[1] << 16);
+        hi[1] = (w0[2] & 0xffffu) | (w0[3] << 16);
+        hi[2] = (w1[0] & 0xffffu) | (w1[1] << 16);
+        hi[3] = (w1[2] & 0xffffu) | (w1[3] << 16);
+        lo[0] = (w0[0] >> 16) | (w0[1] & 0xffff0000u);
+        lo[1] = (w0[2] >> 16) | (w0[3] & 0xffff0000u);
+        lo[2] = (w1[0] >> 16) | (w1[1] & 0xffff0000u);
+        lo[3] = (w1[2] >> 16) | (w1[3] & 0xffff0000u);
+        u4* dst = reinterpret_cast<u4*>(to + pair_at(rows, row0 + row, col0 + c8 * 8));
+        dst[0] = hi;
+        dst[1] = lo;
+    }
+    __builtin_amdgcn_wave_barrier();
+}
+
+// SPLIT: GRAM with its sums in parts (a kernel of its own: in one with the others it cost those 10 %)
+template <class C, Kind KIND, bool SPLIT>
 __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, float ca, float cb, float cc) {
     // arrays of their own, so that the compiler can tell a load into one from reads of another
     __shared__ __attribute__((aligned(128))) char s_ring0[C::STAGE];
@@ -296,8 +354,8 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
     local = xcd * q8 + (xcd < r8 ? xcd : r8) + local / kXcds;
     const unsigned tm = (unsigned(j.mp) + C::BT - 1) / C::BT, tn = (unsigned(j.np) + C::BT - 1) / C::BT;
     constexpr bool SYM = KIND == GRAM || KIND == POLY;
-    const unsigned tiles = SYM ? tm * (tm + 1) / 2 : tm * tn;
-    const unsigned item = local / tiles, tile = local % tiles;
+    const unsigned tiles = SYM ? tm * (tm + 1) / 2 : tm * tn, splits = SPLIT ? j.splits : 1;
+    const unsigned tile = local % tiles, part = SPLIT ? local / tiles % splits : 0, item = local / tiles / splits;
     unsigned ti, tj;
     if (SYM) {                                       // tile = ti (ti + 1) / 2 + tj, tj <= ti
         ti = unsigned((sqrtf(8.0f * float(tile) + 1.0f) - 1.0f) * 0.5f);
@@ -329,9 +387,11 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
         if (r > most) r = most;
         off[l] = (slab * (second ? rows_q : rows_p) + r) * 64 + ((lane & 3) ^ (lane >> 4 & 3)) * 16;
     }
-    const char* pb = p + size_t(i0) * 64;
-    const char* qb = q + size_t(j0) * 64;
     const size_t stage_p = size_t(C::F) * rows_p * 64, stage_q = size_t(C::F) * rows_q * 64;
+    const unsigned all_stages = k / (16 * C::F), each = (all_stages + splits - 1) / splits, stage0 = part * each;      // k is a multiple of 64
+    const unsigned stages = all_stages - stage0 < each ? all_stages - stage0 : each;
+    const char* pb = p + size_t(i0) * 64 + stage0 * stage_p;
+    const char* qb = q + size_t(j0) * 64 + stage0 * stage_q;
     auto load = [&](char* buf, unsigned stage) {
 #pragma unroll
         for (int l = 0; l < C::LOADS; ++l) {
@@ -390,7 +450,6 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
     typedef std::integral_constant<int, int(kAhead) - 1> Full;
     typedef std::integral_constant<int, 1> One;
     typedef std::integral_constant<int, 0> None;
-    const unsigned stages = k / (16 * C::F);         // k is a multiple of 64, F of 1, 2 or 4
     // What the epilogue adds to the sums.  A wave of few tiles asks for it now: at the end it would wait for it.
     auto mine = [&](int tile) { return C::KG == 1 || unsigned(tile) % C::KG == group; };
     const char* addend = KIND == POLY ? buf_a(j, work) : buf_y(j, work, from);
@@ -538,14 +597,62 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
         __syncthreads();
     }
 
+    // A split sum: every part leaves its tile, and the block that is last to do so adds them in their order and goes
+    // on alone.  They lie where the next X and Y will.
+    if (SPLIT && splits > 1) {
+        constexpr unsigned kSide = C::BT / 32;
+        float* parts = reinterpret_cast<float*>(buf_x(j, work, from ^ 1)) + size_t(tile) * splits * kSide * kSide * 1024;
+        auto each_own = [&](auto what) {
+#pragma unroll
+            for (int a = 0; a < C::TM; ++a)
+#pragma unroll
+                for (int b = 0; b < C::TN; ++b)
+                    if (mine(a * C::TN + b) && i0 + wm + a * 32 < rows_p && j0 + wn + b * 32 < rows_q)
+                        what(acc[a][b], ((wm / 32 + a) * kSide + wn / 32 + b) * 1024 + lane * 4);
+        };
+        each_own([&](v16f& sums, unsigned at) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const v4f v = {sums[4 * e], sums[4 * e + 1], sums[4 * e + 2], sums[4 * e + 3]};
+                *reinterpret_cast<v4f*>(parts + size_t(part) * kSide * kSide * 1024 + at + e * 256) = v;
+            }
+        });
+        // The waves' stores have reached this XCD's L2 at the barrier; one thread makes them visible to the others,
+        // and drops what this XCD holds of theirs (by every wave: 361 instead of NNN us for 256 x 4096).
+        __builtin_amdgcn_s_waitcnt(0x0F70);
+        __syncthreads();
+        unsigned* told = reinterpret_cast<unsigned*>(s_ring0);
+        if (threadIdx.x == 0) {
+            __threadfence();
+            const unsigned before = atomicAdd(counters(work) + tile, 1u);
+            if (before == splits - 1) {
+                atomicExch(counters(work) + tile, 0u);                              // for the next launch
+                __threadfence();
+            }
+            *told = before;
+        }
+        __syncthreads();
+        if (*told != splits - 1) return;
+        __syncthreads();                             // the ring is written again below
+        each_own([&](v16f& sums, unsigned at) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sums[e] = 0.0f;
+            for (unsigned n = 0; n < splits; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const v4f v = *reinterpret_cast<const v4f*>(parts + size_t(n) * kSide * kSide * 1024 + at + e * 256);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) sums[4 * e + x] += v[x];
+                }
+        });
+    }
+
     // accumulator register e of a lane: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32 of its 32 x 32 tile
     const bool mirror = !SYM || ti != tj;            // a tile on the diagonal is its own mirror image
     char* direct = KIND == GRAM ? buf_a(j, work) : KIND == POLY ? buf_b(j, work) : buf_x(j, work, from ^ 1);
     char* turned = KIND == GRAM ? buf_a(j, work) : KIND == POLY ? buf_b(j, work) : buf_y(j, work, from ^ 1);
     uint32_t* s_turn = reinterpret_cast<uint32_t*>(piece(wave));       // a 32 x 32 tile per wave is turned in LDS
     const unsigned half = lane >> 5, col = lane & 31;
-    // four words of a row, placed so that rows r and r + 8, and one column of 16 rows, lie in all 64 banks
-    auto turn_at = [](unsigned row, unsigned four) { return (row ^ (row >> 3 & 1)) * 32 + ((four ^ (row >> 1)) & 7) * 4; };
 #pragma unroll
     for (int a = 0; a < C::TM; ++a)
 #pragma unroll
@@ -559,15 +666,8 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
             if (!mine(a * C::TN + b) || gi >= rows_p || gj >= rows_q) continue;     // wave-uniform; rows are multiples of 64
 #pragma unroll
             for (int side = 0; side < 2; ++side) {
-                // rows 16 side + 8 half + 0 .. 7 of the tile in this lane, after the halves have exchanged four
                 float v[8];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[a][b][side * 8 + e]),
-                                                                    __float_as_uint(acc[a][b][side * 8 + 4 + e]), false, false);
-                    v[e] = __uint_as_float(w[0]);
-                    v[4 + e] = __uint_as_float(w[1]);
-                }
+                exchange(acc[a][b], side, v);
                 const unsigned x0 = gi + side * 16 + half * 8;
                 if (KIND == GRAM) {
 #pragma unroll
@@ -588,13 +688,8 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
                     continue;
                 }
                 h8 hi, lo;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    hi[e] = _Float16(v[e]);
-                    lo[e] = _Float16(v[e] - float(hi[e]));
-                    s_turn[turn_at(side * 16 + half * 8 + e, col >> 2) + (col & 3)] =
-                        uint32_t(__builtin_bit_cast(uint16_t, _Float16(hi[e]))) | (uint32_t(__builtin_bit_cast(uint16_t, _Float16(lo[e]))) << 16);
-                }
+                pairs_of(v, &hi, &lo);
+                put_to_turn(s_turn, side, lane, hi, lo);
                 if (mirror) {
                     h8* dst = reinterpret_cast<h8*>(turned + pair_at(rows_q, gj + col, x0));
                     dst[0] = hi;
@@ -602,28 +697,123 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
                 }
             }
             if (KIND == LAST) continue;
-            // a wave reads back only what it wrote itself
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const unsigned row = lane & 31, c8 = 2 * h + half;
-                const u4 w0 = *reinterpret_cast<const u4*>(s_turn + turn_at(row, 2 * c8));
-                const u4 w1 = *reinterpret_cast<const u4*>(s_turn + turn_at(row, 2 * c8 + 1));
-                u4 hi, lo;
-                hi[0] = (w0[0] & 0xffffu) | (w0[1] << 16);
-                hi[1] = (w0[2] & 0xffffu) | (w0[3] << 16);
-                hi[2] = (w1[0] & 0xffffu) | (w1[1] << 16);
-                hi[3] = (w1[2] & 0xffffu) | (w1[3] << 16);
-                lo[0] = (w0[0] >> 16) | (w0[1] & 0xffff0000u);
-                lo[1] = (w0[2] >> 16) | (w0[3] & 0xffff0000u);
-                lo[2] = (w1[0] >> 16) | (w1[1] & 0xffff0000u);
-                lo[3] = (w1[2] >> 16) | (w1[3] & 0xffff0000u);
-                u4* dst = reinterpret_cast<u4*>(direct + pair_at(rows_p, gi + row, gj + c8 * 8));
-                dst[0] = hi;
-                dst[1] = lo;
-            }
-            __builtin_amdgcn_wave_barrier();
+            store_turned(s_turn, lane, direct, rows_p, gi, gj);
         }
+}
+
+// ------------------------------------------------------------------------------- the last two products as one
+// Up to 256 rows: Z = A X, then X' = a X + b Z + c A Z, without B.  A block takes 32 columns of X through both;
+// a wave holds its 32 rows of A in registers, Z goes round the block's waves through LDS.  For twice the
+// multiplications of B X a step is a launch shorter, which is most of its time when X is small.
+constexpr int kJointRows = 128, kJointSteps = kJointRows / 16, kJointWaves = kJointRows / 32;
+template <bool END>
+__global__ __launch_bounds__(kJointWaves * 64) void joint_products(Table t, int from, float ca, float cb, float cc) {
+    // [16 rows of X or Z][32 columns][8 hi, 8 lo, 8 hi, 8 lo], the 16-byte units as in the ring of pair_product
+    __shared__ __attribute__((aligned(128))) char s_x[kJointSteps * 2048];
+    __shared__ __attribute__((aligned(128))) char s_z[kJointSteps * 2048];
+    const int which = job_of(t, blockIdx.x);
+    const Job& j = t.job[which];
+    const unsigned local = blockIdx.x - t.first[which], stripes = unsigned(j.np) / 32, item = local / stripes, j0 = (local % stripes) * 32;
+    char* work = j.work + item * j.work_stride;
+    const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+    const unsigned mp = unsigned(j.mp), np = unsigned(j.np), steps = mp / 16, i0 = wave * 32;
+    const bool rows_here = i0 < mp;                  // wave-uniform
+    const char* y = buf_y(j, work, from);
+    for (unsigned u = wave; u < 2 * steps; u += kJointWaves) {                      // 16 columns of 16 rows
+        const unsigned c = (u & 1) * 16 + (lane >> 2);
+        lds_load(y + (size_t(u >> 1) * np + j0 + c) * 64 + ((lane & 3) ^ (lane >> 4 & 3)) * 16, s_x + u * 1024);
+    }
+    h8 a[kJointSteps][2], old[2][2];
+    if (rows_here) {
+        const char* rows = buf_a(j, work) + (i0 + col) * 64 + half * 32;
+#pragma unroll
+        for (int p = 0; p < kJointSteps; ++p)
+            if (unsigned(p) < steps) {
+                a[p][0] = reinterpret_cast<const h8*>(rows + size_t(p) * mp * 64)[0];
+                a[p][1] = reinterpret_cast<const h8*>(rows + size_t(p) * mp * 64)[1];
+            }
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            const h8* x = reinterpret_cast<const h8*>(y + pair_at(np, j0 + col, i0 + side * 16 + half * 8));
+            old[side][0] = x[0];
+            old[side][1] = x[1];
+        }
+    }
+    const size_t step_x = j.tall ? 1 : size_t(j.cols), step_y = j.tall ? size_t(j.cols) : 1;
+    const size_t first = item * j.stride + i0 * step_x + j0 * step_y, of_lane = half * 8 * step_x + col * step_y;
+    auto inside = [&](int side, int e) { return rows_here && j0 + col < unsigned(j.n) && i0 + side * 16 + half * 8 + e < unsigned(j.m); };
+    float was[2][8];
+    if (END && j.param) {
+#pragma unroll
+        for (int side = 0; side < 2; ++side)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (inside(side, e)) was[side][e] = (j.param + of_lane)[first + (side * 16 + e) * step_x];
+    }
+    const unsigned frag = col * 64, turn = lane >> 2 & 3;
+    // this wave's rows of A times what lies in `in`, the three terms apart: their chains of sums run side by side
+    auto multiply = [&](const char* in) {
+        v16f term[3];
+#pragma unroll
+        for (int n = 0; n < 3; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) term[n][e] = 0.0f;
+#pragma unroll
+        for (int p = 0; p < kJointSteps; ++p)
+            if (unsigned(p) < steps) {
+                const h8 hi = *reinterpret_cast<const h8*>(in + p * 2048 + frag + ((half * 2) ^ turn) * 16);
+                const h8 lo = *reinterpret_cast<const h8*>(in + p * 2048 + frag + ((half * 2 + 1) ^ turn) * 16);
+                term[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[p][0], hi, term[0], 0, 0, 0);
+                term[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[p][0], lo, term[1], 0, 0, 0);
+                term[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[p][1], hi, term[2], 0, 0, 0);
+            }
+        return term[0] + (term[1] + term[2]);
+    };
+    __builtin_amdgcn_s_waitcnt(0x0F70);              // what this wave asked for has landed, in LDS too
+    __syncthreads();
+    v16f z{};
+    float zv[2][8];
+    if (rows_here) {
+        z = multiply(s_x);
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            exchange(z, side, zv[side]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) zv[side][e] *= 1.0f / kScaleA;              // Z times kScaleX
+            h8 hi, lo;
+            pairs_of(zv[side], &hi, &lo);
+            char* to = s_z + (wave * 2 + side) * 2048 + frag;
+            *reinterpret_cast<h8*>(to + ((half * 2) ^ turn) * 16) = hi;
+            *reinterpret_cast<h8*>(to + ((half * 2 + 1) ^ turn) * 16) = lo;
+        }
+    }
+    __syncthreads();                                 // Z is there, and nobody reads X any more
+    if (!rows_here) return;
+    const v16f az = multiply(s_z);
+    uint32_t* s_turn = reinterpret_cast<uint32_t*>(s_x + wave * 4096);
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+        float v[8];
+        exchange(az, side, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float x = ca * (float(old[side][0][e]) + float(old[side][1][e]));
+            v[e] = x + (cb * zv[side][e] + v[e] * (cc / kScaleA));
+        }
+        if (END) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (inside(side, e)) (j.out + of_lane)[first + (side * 16 + e) * step_x] = result_of(t, j, was[side][e], v[e] * (1.0f / kScaleX));
+            continue;
+        }
+        h8 hi, lo;
+        pairs_of(v, &hi, &lo);
+        put_to_turn(s_turn, side, lane, hi, lo);
+        h8* dst = reinterpret_cast<h8*>(buf_y(j, work, from ^ 1) + pair_at(np, j0 + col, i0 + side * 16 + half * 8));
+        dst[0] = hi;
+        dst[1] = lo;
+    }
+    if (!END) store_turned(s_turn, lane, buf_x(j, work, from ^ 1), mp, i0, j0);
 }
 
 // ------------------------------------------------------------------------------- narrow matrices
@@ -1138,55 +1328,85 @@ unsigned full_tiles(const Job& j, unsigned bt) { return ((unsigned(j.mp) + bt - 
 // A parameter's update takes a block `param` us more: a large tile's wave has no registers to ask for all of
 // its part before it has its sums (784 x 2048, 2048 x 2048, 2048 x 4096 and 4096 x 1001 together: tiles of 256
 // in 198 us without and 281 with it, of 128 in 220 and 251).
+struct Pick {
+    int tile;
+    unsigned splits;
+};
+constexpr unsigned kMostSplits = 64, kLeastSum = 256;
+// us: what joining takes a block; per float of every part that it adds; per block of the launch, for the
+// fences go through an XCD's L2 one after the other; and per float that the blocks leave
+constexpr double kJoin = 3.0, kJoinFloat = 4e-5, kJoinBlock = 0.019, kLeaveFloat = 2e-6;
+// Parts of a product's sums, at most `most`, kLeastSum terms or more each, as far as counters and the next X's
+// place reach
+unsigned splits_of(const Job& j, int tile, int k, unsigned most) {
+    const unsigned stage = tile == 256 ? 16 : tile >= 128 ? 32 : 64, stages = unsigned(k) / stage;
+    unsigned n = unsigned(k) / kLeastSum < most ? unsigned(k) / kLeastSum : most;
+    if (n <= 1) return 1;
+    const size_t tiles = sym_tiles(j, unsigned(tile)), room = tiles <= size_t(kCounters) ? 2 * pairs_xy(j) / (tiles * tile * tile * 4) : 1;
+    if (n > room) n = unsigned(room);
+    if (n <= 1) return 1;
+    const unsigned each = (stages + n - 1) / n;
+    return (stages + each - 1) / each;
+}
+struct Choice {
+    int tile, resident;                               // blocks per CU (by LDS)
+    double fixed, per_k, busy, param;
+};
+// when the blocks of a launch are done, in us; the matrices are sorted, longest sums first
 template <class F, class K>
-int pick_tile(const Table& t, F tiles, K k, bool params = false) {
-    const size_t cus = size_t(compute_units() > 0 ? compute_units() : 256);
-    struct Choice {
-        int tile, resident;                           // blocks per CU (by LDS)
-        double fixed, per_k, busy, param;
-    };
-    const Choice choices[6] = {{256, 1, 21.0, 48.0, 1.6, 50.0}, {192, 1, 18.0, 31.0, 1.5, 30.0}, {128, 1, 12.0, 14.0, 1.5, 10.0},
-                               {96, 1, 6.0, 10.6, 1.3, 10.0},   {64, 1, 5.5, 4.6, 1.3, 4.0},     {32, 2, 5.2, 2.9, 1.3, 2.0}};
-    int best = 0;
-    double least = 1e300;
-    for (const Choice& c : choices) {
-        // the places for a block, by the time at which they fall free: a few levels, ascending
-        struct Level {
-            double free_at;
-            size_t places;
-        } level[2 * kMaxJobs + 2] = {{0.0, cus * size_t(c.resident)}};
-        int levels = 1;
-        const size_t places = level[0].places;
-        double sum = 0, done = 0;
-        for (int j = 0; j < t.jobs; ++j) {            // longest first: by_k() has sorted them
-            size_t blocks = size_t(t.job[j].count) * tiles(t.job[j], unsigned(c.tile));
-            const double each = c.fixed + c.per_k * double(k(t.job[j])) / 1024.0 + (params ? c.param : 0.0);
-            sum += double(blocks) * each;
-            const size_t rounds = blocks / places;
-            blocks %= places;
-            for (int l = 0; l < levels; ++l) level[l].free_at += double(rounds) * each;
-            while (blocks) {                          // fewer than the places: each is taken once at most
-                Level first = level[0];
-                const size_t taken = blocks < first.places ? blocks : first.places;
-                blocks -= taken;
-                level[0].places -= taken;
-                if (!level[0].places) {
-                    --levels;
-                    for (int l = 0; l < levels; ++l) level[l] = level[l + 1];
-                }
-                int at = levels++;
-                for (; at > 0 && level[at - 1].free_at > first.free_at + each; --at) level[at] = level[at - 1];
-                level[at] = {first.free_at + each, taken};
+double estimate(const Table& t, const Choice& c, unsigned most_splits, F tiles, K k, bool params) {
+    // the places for a block, by the time at which they fall free: a few levels, ascending
+    const size_t places = size_t(compute_units() > 0 ? compute_units() : 256) * size_t(c.resident);
+    struct Level {
+        double free_at;
+        size_t places;
+    } level[2 * kMaxJobs + 2] = {{0.0, places}};
+    int levels = 1;
+    double sum = 0, done = 0, joins = 0;
+    for (int j = 0; j < t.jobs; ++j) {
+        const unsigned splits = splits_of(t.job[j], c.tile, k(t.job[j]), most_splits);
+        size_t blocks = size_t(t.job[j].count) * tiles(t.job[j], unsigned(c.tile)) * splits;
+        const double each = c.fixed + c.per_k * double(k(t.job[j])) / 1024.0 / splits + (params ? c.param : 0.0) +
+                            (splits > 1 ? kJoin + splits * (c.tile * c.tile) * kJoinFloat : 0.0);
+        if (splits > 1) joins += double(blocks) * (kJoinBlock + c.tile * c.tile * kLeaveFloat);
+        sum += double(blocks) * each;
+        const size_t rounds = blocks / places;
+        blocks %= places;
+        for (int l = 0; l < levels; ++l) level[l].free_at += double(rounds) * each;
+        while (blocks) {                              // fewer than the places
+            const Level first = level[0];
+            const size_t taken = blocks < first.places ? blocks : first.places;
+            blocks -= taken;
+            level[0].places -= taken;
+            if (!level[0].places) {
+                --levels;
+                for (int l = 0; l < levels; ++l) level[l] = level[l + 1];
             }
-        }
-        for (int l = 0; l < levels; ++l)
-            if (level[l].free_at > done) done = level[l].free_at;
-        const double cost = done * (1.0 + (c.busy - 1.0) * sum / (done * double(places)));
-        if (cost < least) {
-            least = cost;
-            best = c.tile;
+            int at = levels++;
+            for (; at > 0 && level[at - 1].free_at > first.free_at + each; --at) level[at] = level[at - 1];
+            level[at] = {first.free_at + each, taken};
         }
     }
+    for (int l = 0; l < levels; ++l)
+        if (level[l].free_at > done) done = level[l].free_at;
+    return joins + done * (1.0 + (c.busy - 1.0) * sum / (done * double(places)));
+}
+template <class F, class K>
+Pick pick_tile(const Table& t, F tiles, K k, bool split = false, bool params = false) {
+    const Choice choices[6] = {{256, 1, 21.0, 48.0, 1.6, 50.0}, {192, 1, 18.0, 31.0, 1.5, 30.0}, {128, 1, 12.0, 14.0, 1.5, 10.0},
+                               {96, 1, 6.0, 10.6, 1.3, 10.0},   {64, 1, 5.5, 4.6, 1.3, 4.0},     {32, 2, 5.2, 2.9, 1.3, 2.0}};
+    unsigned most = split ? unsigned(k(t.job[0])) / kLeastSum : 1;
+    if (most > kMostSplits) most = kMostSplits;
+    Pick best{};
+    double least = 1e300;
+    for (const Choice& c : choices)
+        for (unsigned splits = 1; splits == 1 || (splits <= most && (c.tile == 32 || c.tile == 64 || c.tile == 128)); splits += splits < 4 ? 1 : splits / 2) {
+            const double cost = estimate(t, c, splits, tiles, k, params);
+            if (cost < least) {
+                least = cost;
+                best = {c.tile, splits};
+            }
+        }
     return best;
 }
 
@@ -1199,13 +1419,16 @@ void by_k(Table* t, K k) {
 int gram_k(const Job& j) { return j.np; }
 int square_k(const Job& j) { return j.mp; }
 
-template <class C, Kind KIND>
+template <class C, Kind KIND, bool SPLIT = false>
 void launch_product(Table* t, int from, const float* c, hipStream_t s) {
-    const unsigned blocks = lay_out(t, [](const Job& j) { return KIND == GRAM || KIND == POLY ? sym_tiles(j, C::BT) : full_tiles(j, C::BT); });
-    hipLaunchKernelGGL((pair_product<C, KIND>), dim3(blocks), dim3(C::THREADS), 0, s, *t, from, c[0], c[1], c[2]);
+    const unsigned blocks = lay_out(t, [](const Job& j) {
+        return KIND == GRAM || KIND == POLY ? sym_tiles(j, C::BT) * (SPLIT ? j.splits : 1) : full_tiles(j, C::BT);
+    });
+    hipLaunchKernelGGL((pair_product<C, KIND, SPLIT>), dim3(blocks), dim3(C::THREADS), 0, s, *t, from, c[0], c[1], c[2]);
 }
 template <Kind KIND>
 void launch_product(int tile, Table* t, int from, const float* c, hipStream_t s) {
+    by_k(t, KIND == GRAM ? gram_k : square_k);
     if (tile == 256) launch_product<Tile256, KIND>(t, from, c, s);
     else if (tile == 192) launch_product<Tile192, KIND>(t, from, c, s);
     else if (tile == 128) launch_product<Tile128, KIND>(t, from, c, s);
@@ -1213,21 +1436,35 @@ void launch_product(int tile, Table* t, int from, const float* c, hipStream_t s)
     else if (tile == 64) launch_product<Tile64, KIND>(t, from, c, s);
     else launch_product<Tile32, KIND>(t, from, c, s);
 }
+void launch_gram(Pick pick, Table* t, int from, const float* c, hipStream_t s) {
+    if (pick.splits == 1) return launch_product<GRAM>(pick.tile, t, from, c, s);
+    by_k(t, gram_k);
+    for (int j = 0; j < t->jobs; ++j) t->job[j].splits = splits_of(t->job[j], pick.tile, t->job[j].np, pick.splits);
+    if (pick.tile == 128) launch_product<Tile128, GRAM, true>(t, from, c, s);
+    else if (pick.tile == 64) launch_product<Tile64, GRAM, true>(t, from, c, s);
+    else launch_product<Tile32, GRAM, true>(t, from, c, s);
+}
 
 int iterate(const char* who, Table* t, int steps, const float* c, hipStream_t s) {
-    by_k(t, square_k);
-    const int poly = pick_tile(*t, sym_tiles, square_k), full = pick_tile(*t, full_tiles, square_k);
-    const int last = pick_tile(*t, full_tiles, square_k, t->job[0].param != nullptr);
     by_k(t, gram_k);
-    const int gram = pick_tile(*t, sym_tiles, gram_k);
+    const Pick gram = pick_tile(*t, sym_tiles, gram_k, true);
+    by_k(t, square_k);
+    const int poly = pick_tile(*t, sym_tiles, square_k).tile, full = pick_tile(*t, full_tiles, square_k).tile,
+              last = pick_tile(*t, full_tiles, square_k, false, t->job[0].param != nullptr).tile;
+    bool joint = true;
+    for (int k = 0; k < t->jobs; ++k) joint = joint && t->job[k].mp <= kJointRows;
     for (int k = 0; k < steps; ++k) {
         const int from = k & 1;
-        by_k(t, gram_k);
-        launch_product<GRAM>(gram, t, from, c, s);
-        by_k(t, square_k);
-        launch_product<POLY>(poly, t, from, c, s);
-        if (k + 1 < steps) launch_product<STEP>(full, t, from, c, s);
-        else launch_product<LAST>(last, t, from, c, s);
+        launch_gram(gram, t, from, c, s);
+        if (joint) {
+            const unsigned blocks = lay_out(t, [](const Job& j) { return unsigned(j.np) / 32; });
+            if (k + 1 < steps) hipLaunchKernelGGL((joint_products<false>), dim3(blocks), dim3(kJointWaves * 64), 0, s, *t, from, c[0], c[1], c[2]);
+            else hipLaunchKernelGGL((joint_products<true>), dim3(blocks), dim3(kJointWaves * 64), 0, s, *t, from, c[0], c[1], c[2]);
+        } else {
+            launch_product<POLY>(poly, t, from, c, s);
+            if (k + 1 < steps) launch_product<STEP>(full, t, from, c, s);
+            else launch_product<LAST>(last, t, from, c, s);
+        }
         const int rc = launched(who);
         if (rc) return rc;
     }

@@ -83,6 +83,81 @@ def test_large_matrices(shape):
     assert 0.6 * np.sqrt(min(shape)) < float(got.norm()) < 1.25 * np.sqrt(min(shape))
 
 
+# the sums of X X^T in parts, joined by the block that is last: few rows, long columns, ragged ends
+LONG = [(128, 20000), (100, 9001), (20001, 130), (256, 16390), (66, 70001), (512, 8200), (64, 9001)]
+
+
+@pytest.mark.parametrize("shape", LONG, ids=lambda s: "%dx%d" % s)
+def test_few_long_rows(shape):
+    import gpu_support as G
+    import torch
+    g = _gradient(*shape, seed=7)
+    got = _ns(G, G.dev(g))
+    _check(got, g)
+    assert torch.equal(_ns(G, G.dev(g)), got)                                          # parts are added in their order
+
+
+def test_few_long_rows_in_a_batch_on_two_streams_and_replayed():
+    """A workspace's counters are back at zero after every product: a second call, a recorded one replayed, and a
+    call at the same time in a workspace of its own give the first one's bits."""
+    import gpu_support as G
+    import torch
+    lib = G.lib()
+    g = _gradient(130, 9000, seed=3, batch=3)
+    x = G.dev(g)
+    size = C.c_size_t()
+    assert lib.ctamd_newton_schulz_workspace(130, 9000, 3, C.byref(size)) == 0
+    work = [_workspace(G, size.value) for _ in range(2)]
+    want = _ns(G, x, work=work[0])
+    for i in range(3):
+        _check(want[i], g[i])
+    streams = [C.c_void_p(), C.c_void_p()]
+    for s in streams:
+        assert lib.ctamd_stream_create(C.byref(s)) == 0
+    out = [torch.empty_like(x) for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for o, w, s in zip(out, work, streams):
+            _ns(G, x, out=o, work=w, stream=s)
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], want) and torch.equal(out[1], want)
+    graph = C.c_void_p()
+    replayed = torch.empty_like(x)
+    torch.cuda.synchronize()
+    assert lib.ctamd_graph_begin(streams[0]) == 0
+    _ns(G, x, out=replayed, work=work[0], stream=streams[0])
+    assert lib.ctamd_graph_end(streams[0], C.byref(graph)) == 0
+    for _ in range(3):
+        replayed.zero_()
+        torch.cuda.synchronize()
+        assert lib.ctamd_graph_launch(graph, streams[0]) == 0
+        _ns(G, x, out=out[1], work=work[1])                                            # the program's own, at the same time
+        torch.cuda.synchronize()
+        assert torch.equal(replayed, want) and torch.equal(out[1], want)
+    assert lib.ctamd_graph_destroy(graph) == 0
+    for s in streams:
+        assert lib.ctamd_stream_destroy(s) == 0
+
+
+def test_a_step_over_few_long_rows():
+    import gpu_support as G
+    import torch
+    r = np.random.default_rng(2)
+    shapes = [(96, 12000), (12001, 100), (128, 64)]
+    host = [((r.standard_normal(s) / 10).astype(np.float32), _gradient(*s, 20 + k), 5 * _gradient(*s, 40 + k), float(0.2 * np.sqrt(max(s))))
+            for k, s in enumerate(shapes)]
+    dev = [tuple(G.dev(v) for v in h[:3]) for h in host]
+    out = [(torch.full_like(p, float("nan")), torch.full_like(p, float("nan"))) for p, _, _ in dev]
+    _muon(G, [(*d, *o, h[3]) for d, o, h in zip(dev, out, host)], _options())
+    for (p, g, m, scale), (new, new_m) in zip(host, out):
+        want, wm, err, merr = O.muon(p, g, m, scale, 0.02, 0.95, 0.01, True, 5)
+        assert np.all(np.abs(new_m.cpu().numpy() - wm) <= merr)
+        assert np.all(np.abs(new.cpu().numpy() - want) <= err), p.shape
+    _muon(G, [(d[0], d[1], d[2], d[0], d[2], h[3]) for d, h in zip(dev, host)], _options())
+    for (p, _, m), (new, new_m) in zip(dev, out):
+        assert torch.equal(p, new) and torch.equal(m, new_m)
+
+
 def test_singular_values_are_driven_towards_one():
     import gpu_support as G
     r = np.random.default_rng(1)
