@@ -618,7 +618,8 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
             }
         });
         // The waves' stores have reached this XCD's L2 at the barrier; one thread makes them visible to the others,
-        // and drops what this XCD holds of theirs (by every wave: 361 instead of NNN us for 256 x 4096).
+        // and drops what this XCD holds of theirs (by every wave: 361 instead of 187 us
+        // for 256 x 4096 in 16 parts).
         __builtin_amdgcn_s_waitcnt(0x0F70);
         __syncthreads();
         unsigned* told = reinterpret_cast<unsigned*>(s_ring0);
@@ -702,9 +703,11 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
 }
 
 // ------------------------------------------------------------------------------- the last two products as one
-// Up to 256 rows: Z = A X, then X' = a X + b Z + c A Z, without B.  A block takes 32 columns of X through both;
+// Up to 128 rows: Z = A X, then X' = a X + b Z + c A Z, without B.  A block takes 32 columns of X through both;
 // a wave holds its 32 rows of A in registers, Z goes round the block's waves through LDS.  For twice the
-// multiplications of B X a step is a launch shorter, which is most of its time when X is small.
+// multiplications of B X a step is a launch shorter: 100 x 100 in 65 instead of 75 us, 128 x 784 in 78 instead
+// of 89, never slower up to 128 x 200000.  With 256 rows a block's CU reads 256 KiB of A and multiplies for all
+// of them: 13.0 us where A A and B X take 5.6 and 6.0.
 constexpr int kJointRows = 128, kJointSteps = kJointRows / 16, kJointWaves = kJointRows / 32;
 template <bool END>
 __global__ __launch_bounds__(kJointWaves * 64) void joint_products(Table t, int from, float ca, float cb, float cc) {
@@ -936,7 +939,7 @@ __global__ __launch_bounds__(C::THREADS) void narrow_product(Table t, int steps,
     const unsigned j0 = stripe * C::STRIPE + wave * 32, gj = j0 + (lane & 31);
     const bool live = j0 < unsigned(j.n);                                          // wave-uniform
     // register e of tile a is element (32 a + 8 (e / 4) + 4 half + e % 4, gj).  Loads go to a place inside the
-    // matrix whatever the register (no branch, all of them on their way at once); 2^20 x 64 has 32-bit places.
+    // matrix whatever the register (no branch, all of them on their way at once); 131072 x 64 has 32-bit places.
     const size_t matrix = item * j.stride;
     const unsigned cols = unsigned(j.cols), down = j.tall ? 1 : cols, across = j.tall ? cols : 1, last_row = unsigned(j.m) - 1;
     const bool in_col = gj < unsigned(j.n);
@@ -1471,10 +1474,10 @@ int iterate(const char* who, Table* t, int steps, const float* c, hipStream_t s)
     return CTAMD_OK;
 }
 
-// Whether the narrow kernels take a matrix: beyond some stripes the blocks' sums of all shares cost more than
-// the separate products' launches.
-constexpr unsigned kMostStripes = 32;
-bool is_narrow(const Job& j) { return j.m <= 64 && stripes_of(j, kLeastStripe) <= kMostStripes; }
+// Whether the narrow kernels take matrices of up to m rows and n columns: with more stripes every block's sum of
+// all stripes' shares costs more than the separate products' launches (narrow and separate, us: 64 x 16384
+// 109 and 132, 64 x 32768 158 and 183, 64 x 65536 264 and 257; 16 x 16384 65 and 127, 16 x 65536 102 and 255).
+bool is_narrow(int m, int n) { return m <= 32 ? n <= 131072 : m <= 64 && n <= 49152; }
 
 template <class C>
 void launch_whole(Table* t, int steps, const float* c, hipStream_t s) {
@@ -1496,15 +1499,14 @@ int run_table(const char* who, Table* t, int steps, const float* c, hipStream_t 
         j.vec = j.cols % 4 == 0 && aligned16(j.grad) && (!j.momentum || (aligned16(j.momentum) && aligned16(j.new_momentum)));
     }
     double bytes = 0, flops = 0;
-    bool narrow = true;
     int most_m = 0, most_n = 0;
     for (int j = 0; j < t->jobs; ++j) {
-        narrow = narrow && is_narrow(t->job[j]);
         if (t->job[j].m > most_m) most_m = t->job[j].m;
         if (t->job[j].n > most_n) most_n = t->job[j].n;
         bytes += (t->job[j].param ? 20.0 : 8.0) * double(t->job[j].stride) * t->job[j].count;
         flops += flops_of(t->job[j], steps);
     }
+    const bool narrow = is_narrow(most_m, most_n);
     if (narrow && (most_m <= 32 ? most_n <= FlatWide::STRIPE : most_n <= Narrow::STRIPE)) {
         if (most_m > 32) launch_whole<Narrow>(t, steps, c, s);
         else if (most_n > Flat::STRIPE) launch_whole<FlatWide>(t, steps, c, s);

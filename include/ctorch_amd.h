@@ -373,7 +373,7 @@ int ctamd_matmul_relu_mask_f32(const float* a, int64_t as0, int64_t as1, const f
  * in memory.  coefficients_host (HOST, may be NULL): a, b, c; NULL stands for 3.4445, -4.7750, 2.0315, which
  * in 5 steps take singular values of 0.005 |g|_F and more to 0.7 - 1.2.  Matrices are held as pairs of f16
  * numbers with 22 bits together (three with 24 where no matrix of the call has more than 32 on its shorter
- * side and 8192 on its longer) and multiplied by the f16 matrix cores with fp32 sums: as close to the
+ * side and 131072 on its longer) and multiplied by the f16 matrix cores with fp32 sums: as close to the
  * iteration in 64 bits as fp32 products are.  That holds while the entries of X stay below 8 and
  * those of A and b A + c A A below 32 (singular values below 4 or so; the given coefficients keep them below
  * 1.3); coefficients beyond 32 are CTAMD_EINVAL.  An update whose norm is far below eps comes out as zero

@@ -84,7 +84,7 @@ def test_large_matrices(shape):
 
 
 # the sums of X X^T in parts, joined by the block that is last: few rows, long columns, ragged ends
-LONG = [(128, 20000), (100, 9001), (20001, 130), (256, 16390), (66, 70001), (512, 8200), (64, 9001)]
+LONG = [(128, 20000), (100, 9001), (20001, 130), (256, 16390), (66, 70001), (512, 8200), (64, 9001), (64, 60001), (30, 60000)]
 
 
 @pytest.mark.parametrize("shape", LONG, ids=lambda s: "%dx%d" % s)
