@@ -19,6 +19,9 @@
 // its number, so that the 16 lanes that the 64 banks serve at once (of a ds_read_b128 per 32 x 16 operand
 // half) meet no bank twice.  Both operands of every product are read along their rows (A and B are symmetric;
 // X is kept with its transpose Y), so one kernel serves all three.
+//
+// Five steps on 4096 x 4096 take 3.7 ms, on 2048 x 2048 0.67: the 1.37 and 0.17 Tflop that symmetry leaves are
+// 370 and 255 Tflop/s, a third of 1110 and 770 on the matrix cores, where a large f16 product reaches 1370.
 #include <algorithm>
 #include <cmath>
 #include <memory>
@@ -861,6 +864,12 @@ __device__ __forceinline__ Parts<N> parts_of(const float (&v)[16]) {
         }
     return r;
 }
+__device__ __forceinline__ v16f zero16() {
+    v16f z;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) z[e] = 0.0f;
+    return z;
+}
 // the products of parts whose places add up to less than N: what is left out is below 2^(-11 N)
 template <int N>
 __device__ __forceinline__ void multiply_parts(v16f& acc, const Parts<N>& p, const Parts<N>& q) {
@@ -870,12 +879,6 @@ __device__ __forceinline__ void multiply_parts(v16f& acc, const Parts<N>& p, con
         for (int sum = N - 1; sum >= 0; --sum)
 #pragma unroll
             for (int i = 0; i <= sum; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p.part[i][s], q.part[sum - i][s], acc, 0, 0, 0);
-}
-__device__ __forceinline__ v16f zero16() {
-    v16f z;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) z[e] = 0.0f;
-    return z;
 }
 // a tile of 32 x 32 floats in memory: [register / 4][lane][register % 4]
 __device__ __forceinline__ void put_tile(float* to, unsigned lane, const float (&v)[16]) {
@@ -899,9 +902,9 @@ template <int ROWS_, int WAVES_>
 struct NarrowCfg {
     static constexpr int ROWS = ROWS_, WAVES = WAVES_, STRIPE = 32 * WAVES_, TILES = ROWS * ROWS, THREADS = 64 * WAVES_;
     static constexpr int N = ROWS == 1 ? 3 : 2;       // parts of a number
-    // ROWS == 1: the waves' shares twice (a wave may be a step ahead of another that still reads).
-    // ROWS == 2: the shares - and in their place, later in a step, the parts of A A - and their sum.
-    static constexpr int SHARES = ROWS == 1 ? 2 * WAVES : WAVES * TILES;
+    // The waves' shares - and in their place, later in a step of ROWS == 2, the parts of A A - and their sum: four
+    // elements to a thread (each wave adding all of them for itself took 24.5 us for 256 x 10, this 20.6).
+    static constexpr int SHARES = ROWS == 1 ? WAVES + 1 : WAVES * TILES;
     static_assert(STRIPE * (32 * ROWS + 1) <= SHARES * int(kTileFloats), "a tall matrix's stripe is turned in the shares' place");
 };
 typedef NarrowCfg<1, 8> Flat;                         // up to 32 x 256
@@ -1100,15 +1103,7 @@ __global__ __launch_bounds__(C::THREADS) void narrow_product(Table t, int steps,
                 put_tile(shares + (wave * TILES + a * ROWS + b) * kTileFloats, lane, v);
             }
     };
-    // The sum of the waves' shares.  One tile: every wave adds them for itself.  Four: a thread adds its
-    // eight elements, into s_sum.
-    auto own_sum = [&](const float* shares, float (&v)[16]) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) add_tile(shares + w * kTileFloats, lane, v);
-    };
-    constexpr unsigned kPerThread = TILES * kTileFloats / C::THREADS / 4;          // vectors of 4 (ROWS == 2)
+    // the sum of shares, four elements of it
     auto joint_sum = [&](const float* shares, unsigned count, size_t stride, unsigned i) {
         v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
         for (unsigned w0 = 0; w0 < count; w0 += 8) {  // eight on their way at once; beyond the last, the last again
@@ -1186,17 +1181,20 @@ __global__ __launch_bounds__(C::THREADS) void narrow_product(Table t, int steps,
 #pragma unroll 1
         for (int s = 0; s < steps; ++s) {
             part_x();
-            float* shares = s_share + (ROWS == 1 ? (s & 1) * WAVES * int(kTileFloats) : 0);
-            put_shares(shares);
+            put_shares(s_share);
+            __syncthreads();
+            for (unsigned i = threadIdx.x; i < TILES * kTileFloats / 4; i += C::THREADS)
+                *reinterpret_cast<v4f*>(s_sum + i * 4) = joint_sum(s_share, WAVES, TILES * kTileFloats, i);
             __syncthreads();
             if (ROWS == 1) {
-                own_sum(shares, a);
-            } else {
 #pragma unroll
-                for (unsigned i = 0; i < kPerThread; ++i)
-                    *reinterpret_cast<v4f*>(s_sum + (threadIdx.x + i * C::THREADS) * 4) =
-                        joint_sum(shares, WAVES, TILES * kTileFloats, threadIdx.x + i * C::THREADS);
-                __syncthreads();
+                for (int e = 0; e < 16; ++e) a[e] = 0.0f;
+                add_tile(s_sum, lane, a);
+            }
+            if (C::THREADS > 512) {                   // 128 registers a lane: the parts are formed again, not kept
+#pragma unroll
+                for (int e = 0; e < 16; ++e) asm volatile("" : "+v"(x[0][e]));
+                part_x();
             }
             step(a);
         }
