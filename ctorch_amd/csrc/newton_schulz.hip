@@ -620,23 +620,23 @@ __global__ __launch_bounds__(C::THREADS) void pair_product(Table t, int from, fl
                 *reinterpret_cast<v4f*>(parts + size_t(part) * kSide * kSide * 1024 + at + e * 256) = v;
             }
         });
-        // The waves' stores have reached this XCD's L2 at the barrier; one thread makes them visible to the others,
-        // and drops what this XCD holds of theirs (by every wave: 361 instead of 187 us
-        // for 256 x 4096 in 16 parts).
+        // The waves' stores have reached this XCD's L2 at the barrier; one thread writes it back for the others to
+        // see (every wave of a block doing so took twice the time for 256 x 4096 in 16 parts).  The wait is
+        // written out: the compiler counts the write-back for nothing and would let the counter overtake it.
         __builtin_amdgcn_s_waitcnt(0x0F70);
         __syncthreads();
         unsigned* told = reinterpret_cast<unsigned*>(s_ring0);
         if (threadIdx.x == 0) {
-            __threadfence();
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             const unsigned before = atomicAdd(counters(work) + tile, 1u);
-            if (before == splits - 1) {
-                atomicExch(counters(work) + tile, 0u);                              // for the next launch
-                __threadfence();
-            }
+            if (before == splits - 1) atomicExch(counters(work) + tile, 0u);       // for the next launch
             *told = before;
         }
         __syncthreads();
         if (*told != splits - 1) return;
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");                          // drops what is held of the others' parts
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();                             // the ring is written again below
         each_own([&](v16f& sums, unsigned at) {
 #pragma unroll
@@ -1336,7 +1336,9 @@ struct Pick {
 constexpr unsigned kMostSplits = 64, kLeastSum = 256;
 // us: what joining takes a block; per float of every part that it adds; per block of the launch, for the
 // fences go through an XCD's L2 one after the other; and per float that the blocks leave
-constexpr double kJoin = 3.0, kJoinFloat = 4e-5, kJoinBlock = 0.019, kLeaveFloat = 2e-6;
+constexpr double kJoin = 3.5, kJoinFloat = 4e-5, kJoinBlock = 0.045, kLeaveFloat = 2e-6;
+// (in parts and not, us: 70 x 3000 100 and 120, 128 x 4096 106 and 144, 128 x 200000 0.89 and 4.36 ms, 256 x 4096 174
+// and 180, 333 x 20000 411 and 590, 512 x 8192 335 and 333)
 // Parts of a product's sums, at most `most`, kLeastSum terms or more each, as far as counters and the next X's
 // place reach
 unsigned splits_of(const Job& j, int tile, int k, unsigned most) {
